@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "capi_cuda.h"
+#include "train.hpp"
 
 namespace
 {
@@ -384,13 +385,16 @@ PyMethodDef kMethods[] = {
 };
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fastcall",
-                       "Collectives on CUDA tensors: argument checks and the library call.", -1,
+                       "Collectives and operators on CUDA tensors: argument checks and the library call.", -1,
                        kMethods, nullptr, nullptr, nullptr, nullptr};
 }  // namespace
 
 PyMODINIT_FUNC PyInit__fastcall()
 {
     PyObject *m = PyModule_Create(&kModule);
-    if (m != nullptr) { PyModule_AddIntConstant(m, "MIXED_DTYPES", kMixedDtypes); }
+    if (m != nullptr) {
+        PyModule_AddIntConstant(m, "MIXED_DTYPES", kMixedDtypes);
+        PyModule_AddFunctions(m, train_methods());
+    }
     return m;
 }
