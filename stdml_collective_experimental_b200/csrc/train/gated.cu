@@ -21,71 +21,175 @@ constexpr int kPieces = 3;
 
 __device__ unsigned int g_status;
 
-// ------------------------------------------------------------ results of a tile
+// ------------------------------------------------------------ what the backward pass needs of g and u
+// Blocks of some columns of a row, both values together.  16-bit types: 24 bits of each, the upper 16 and the next 8
+// apart (16 bits would put two more roundings as large as a result's own into every gradient; 32 would cost a
+// third more bytes).  32-bit types: all of them.
 template <typename T>
-__device__ __forceinline__ void store16(T *to, const float (&v)[16], long long left, bool vec)
+struct Saved {
+    static constexpr int kCols = 16;
+    static constexpr int kBytes = sizeof(T) == 4 ? 128 : 96;  // g, u in 32 bits | upper g, upper u, lower g, lower u
+    __host__ __device__ static long long row_bytes(long long ffn) { return (ffn + kCols - 1) / kCols * kBytes; }
+};
+
+// ------------------------------------------------------------ results of a tile
+// An epilogue warp has 32 rows of a tile, one to a thread; through 32 rows of 128 bytes in shared memory they reach
+// global memory 32 bytes and more in a row (stores of 16 bytes from 32 rows at a time took longer than the products).
+// Pieces of 16 bytes lie swizzled, so that neither side meets bank conflicts.
+__device__ __forceinline__ uint4 *piece_at(unsigned char *mem, int row, int piece)
 {
-    if (vec && left >= 16) {
-        if constexpr (sizeof(T) == 4) {
+    return reinterpret_cast<uint4 *>(mem + 128 * row + 16 * (piece ^ (row & 7)));
+}
+
+template <typename T>
+__device__ __forceinline__ void put16(unsigned char *mem, int row, int piece, const float (&v)[16])
+{
+    constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                reinterpret_cast<float4 *>(to)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-            }
-        } else {
-            __align__(16) T t[16];
+    for (int j = 0; j < 16 / kPer; ++j) {
+        __align__(16) T t[kPer];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { t[i] = from_f32<T>(v[i]); }
-            reinterpret_cast<uint4 *>(to)[0] = reinterpret_cast<const uint4 *>(t)[0];
-            reinterpret_cast<uint4 *>(to)[1] = reinterpret_cast<const uint4 *>(t)[1];
+        for (int i = 0; i < kPer; ++i) { t[i] = from_f32<T>(v[kPer * j + i]); }
+        *piece_at(mem, row, piece + j) = *reinterpret_cast<const uint4 *>(t);
+    }
+}
+
+// Where kPieces pieces of each of 32 rows go, 32 / kPieces rows at a time: to + r * pitch + 16 * piece.
+template <int kPieces>
+struct RowsOut {
+    unsigned char *to;  // this thread's first piece
+    long long step;     // from one of its rows to the next
+    int left;           // rows of this thread's row and those below
+
+    __device__ __forceinline__ RowsOut(void *base, long long pitch, int row0, int m)
+    {
+        const int r = (threadIdx.x & 31) / kPieces;
+        to = static_cast<unsigned char *>(base) + (row0 + r) * pitch + 16 * (threadIdx.x % kPieces);
+        step = 32 / kPieces * pitch;
+        left = m - row0 - r;
+    }
+    // From pieces `first` on in shared memory, `bytes` further on in each row.
+    __device__ __forceinline__ void copy(unsigned char *mem, int first, long long bytes) const
+    {
+        const int r = (threadIdx.x & 31) / kPieces, q = threadIdx.x % kPieces;
+        unsigned char *at = to + bytes;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k, at += step) {
+            if (32 / kPieces * k < left) { *reinterpret_cast<uint4 *>(at) = *piece_at(mem, r + 32 / kPieces * k, first + q); }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (i < left) { to[i] = from_f32<T>(v[i]); }
+    }
+};
+
+// The same for rows at any address, element by element: columns [col, col + kBytes / sizeof(T)) of a result of n.
+template <typename T, int kBytes>
+__device__ __noinline__ void rows_out_any(unsigned char *mem, T *out, int row0, int m, long long n, long long col)
+{
+    constexpr int kWords = kBytes / 4;
+    for (int i = threadIdx.x & 31; i < 32 * kWords; i += 32) {
+        const int r = i / kWords, q = i % kWords;
+        const long long c = col + q * static_cast<int>(4 / sizeof(T));
+        if (row0 + r >= m || c >= n) { continue; }
+        const uint32_t word = reinterpret_cast<const uint32_t *>(piece_at(mem, r, q / 4))[q % 4];
+        T *to = out + (row0 + r) * n + c;
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<uint32_t *>(to) = word;
+        } else if (c + 1 < n && reinterpret_cast<uintptr_t>(to) % 4 == 0) {
+            *reinterpret_cast<uint32_t *>(to) = word;
+        } else {
+            reinterpret_cast<uint16_t *>(to)[0] = static_cast<uint16_t>(word);
+            if (c + 1 < n) { reinterpret_cast<uint16_t *>(to)[1] = static_cast<uint16_t>(word >> 16); }
         }
     }
 }
 
-// g and u of 128 columns side by side in a tile: h, and what the backward pass needs of them.
+// g and u of the same columns side by side in a tile: h, and what the backward pass needs of them.
 template <typename T, int kAct>
 struct GatedTile {
     T *h;
     const T *b_gate, *b_up;
-    float *saved;  // g, u: [2][tokens][pitch]
-    long long pitch;
-    bool vec;
+    unsigned char *saved;
+    bool vec_h, vec_b;
 
-    __device__ __forceinline__ void tile(const Product &p, long long m0, long long nt, int, int warp, uint32_t tmem) const
+    __device__ __forceinline__ void add_bias(const T *bias, long long col, int n, float (&v)[16]) const
     {
-        const long long row = m0 + 32 * (warp & 3) + (threadIdx.x & 31);
-        const int half = warp >> 2;
-        tmem += (32u * (warp & 3) << 16) + 64 * half;
+        if (vec_b && col + 16 <= n) {
+            constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+            for (int j = 0; j < 16 / kPer; ++j) {
+                __align__(16) T t[kPer];
+                *reinterpret_cast<uint4 *>(t) = reinterpret_cast<const uint4 *>(bias + col)[j];
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) { v[kPer * j + i] += to_f32(t[i]); }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { v[i] += col + i < n ? to_f32(bias[col + i]) : 0.f; }
+        }
+    }
+    // The upper 16 bits of 16 values into two pieces, the next 8 into one.
+    __device__ __forceinline__ static void keep24(unsigned char *mem, int row, int upper, int lower, const float (&v)[16])
+    {
+        uint32_t up[8], low[4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            up[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t a = __byte_perm(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), 0x0051),
+                           b = __byte_perm(__float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]), 0x0051);
+            low[i] = __byte_perm(a, b, 0x5410);
+        }
+        *piece_at(mem, row, upper) = make_uint4(up[0], up[1], up[2], up[3]);
+        *piece_at(mem, row, upper + 1) = make_uint4(up[4], up[5], up[6], up[7]);
+        *piece_at(mem, row, lower) = make_uint4(low[0], low[1], low[2], low[3]);
+    }
+
+    template <int kN, typename Source>
+    __device__ __forceinline__ void tile(const Product &p, int, int row0, int nt, int, int slice, unsigned char *mem,
+                                         const Source &from) const
+    {
+        constexpr int kCols = Saved<T>::kCols, kPasses = Shape<kN>::kBlocks / 2, kPieces = sizeof(T);
+        const int lane = threadIdx.x & 31;
+        const long long first = nt * (kN / 2ll) + kPasses * kCols * slice;
+        const RowsOut<kPieces> rows_h(h + first, p.n * static_cast<long long>(sizeof(T)), row0, p.m);
+        const RowsOut<kPieces> rows_s(saved + first / kCols * Saved<T>::kBytes, Saved<T>::row_bytes(p.n), row0, p.m);
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-            const long long col = nt * 128 + 64 * half + 16 * c;
+        for (int b = 0; b < kPasses; ++b) {
+            const long long col = first + kCols * b;
             if (col >= p.n) { break; }
             float g[16], u[16];
-            tmem_load16(tmem + 16 * c, g);
-            tmem_load16(tmem + 128 + 16 * c, u);
-            tmem_loaded(g);
-            tmem_loaded(u);
-            if (row < p.m) {
-                if (b_gate != nullptr) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (col + i < p.n) {
-                            g[i] += to_f32(b_gate[col + i]);
-                            u[i] += to_f32(b_up[col + i]);
-                        }
-                    }
+            from.load(b, g);
+            from.load(kPasses + b, u);
+            from.loaded(g);
+            from.loaded(u);
+            if (b_gate != nullptr) {
+                add_bias(b_gate, col, p.n, g);
+                add_bias(b_up, col, p.n, u);
+            }
+            if (saved != nullptr) {
+                if constexpr (sizeof(T) == 4) {
+                    put16<T>(mem, lane, 0, g);
+                    put16<T>(mem, lane, 4, u);
+                } else {
+                    keep24(mem, lane, 2, 6, g);
+                    keep24(mem, lane, 4, 7, u);
                 }
-                if (saved != nullptr) {
-                    store16(saved + row * pitch + col, g, 16, true);
-                    store16(saved + (p.m + row) * pitch + col, u, 16, true);
-                }
+                __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) { u[i] *= act<kAct>(g[i]); }
-                store16(h + row * p.n + col, u, p.n - col, vec);
+                for (int j = 0; j < Saved<T>::kBytes / (16 * kPieces); ++j) {
+                    rows_s.copy(mem, (sizeof(T) == 4 ? 0 : 2) + kPieces * j, Saved<T>::kBytes * b + 16 * kPieces * j);
+                }
+                if constexpr (sizeof(T) == 4) { __syncwarp(); }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { u[i] *= act<T, kAct>(g[i]); }
+            put16<T>(mem, lane, 0, u);
+            __syncwarp();
+            if (vec_h && col + kCols <= p.n) {
+                rows_h.copy(mem, 0, kCols * static_cast<int>(sizeof(T)) * b);
+            } else {
+                rows_out_any<T, kCols * sizeof(T)>(mem, h, row0, p.m, p.n, col);
             }
             __syncwarp();
         }
@@ -94,23 +198,34 @@ struct GatedTile {
 
 template <typename T>
 struct PlainTile {
-    T *out[2];  // of each z
+    T *out[2][2];  // [product][z]
     bool vec;
 
-    __device__ __forceinline__ void tile(const Product &p, long long m0, long long nt, int z, int warp, uint32_t tmem) const
+    template <int kN, typename Source>
+    __device__ __forceinline__ void tile(const Product &p, int product, int row0, int nt, int z, int slice, unsigned char *mem,
+                                         const Source &from) const
     {
-        const long long row = m0 + 32 * (warp & 3) + (threadIdx.x & 31);
-        const int half = warp >> 2;
-        tmem += (32u * (warp & 3) << 16) + 128 * half;
-        T *to = out[z] + row * p.n;
+        constexpr int kOf = Shape<kN>::kValues, kCols = kOf * sizeof(T) > 128 ? 128 / sizeof(T) : kOf;
+        T *to = product == 0 ? (z == 0 ? out[0][0] : out[0][1]) : (z == 0 ? out[1][0] : out[1][1]);
+        const long long first = nt * static_cast<long long>(kN) + kOf * slice;
+        const RowsOut<kCols * static_cast<int>(sizeof(T)) / 16> rows(to + first, p.n * static_cast<long long>(sizeof(T)), row0, p.m);
 #pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-            const long long col = nt * kTileN + 128 * half + 16 * c;
+        for (int c = 0; c < kOf; c += kCols) {
+            const long long col = first + c;
             if (col >= p.n) { break; }
-            float v[16];
-            tmem_load16(tmem + 16 * c, v);
-            tmem_loaded(v);
-            if (row < p.m) { store16(to + col, v, p.n - col, vec); }
+#pragma unroll
+            for (int b = 0; b < kCols / 16; ++b) {
+                float v[16];
+                from.load(c / 16 + b, v);
+                from.loaded(v);
+                put16<T>(mem, threadIdx.x & 31, b * static_cast<int>(sizeof(T)), v);
+            }
+            __syncwarp();
+            if (vec && col + kCols <= p.n) {
+                rows.copy(mem, 0, c * static_cast<int>(sizeof(T)));
+            } else {
+                rows_out_any<T, kCols * sizeof(T)>(mem, to, row0, p.m, p.n, col);
+            }
             __syncwarp();
         }
     }
@@ -159,11 +274,59 @@ constexpr int kGradRows = 64, kGradCols = 256;  // of a block: 8 rows of 32 thre
 struct GateGrad {
     const void *dh;
     long long dh_row;
-    const float *saved;
+    const unsigned char *saved;
     long long tokens, ffn, pitch;
     uint16_t *d;      // [gate, up][pieces][tokens][pitch]
     float *partial;   // [row blocks][gate, up][ffn]; null: no sums
     bool vec;
+};
+
+// 8 columns of a row of dh, and the saved g and u.
+template <typename T>
+struct GateGradRow {
+    __align__(16) T dh[8];
+    __align__(16) uint32_t g[sizeof(T) == 4 ? 8 : 4], u[sizeof(T) == 4 ? 8 : 4];
+    uint2 low_g, low_u;
+
+    __device__ __forceinline__ void load(const GateGrad &a, long long r, long long col)
+    {
+        const T *from = static_cast<const T *>(a.dh) + r * a.dh_row + col;
+        if (a.vec) {  // (and so ffn is a multiple of 16 bytes)
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(8 * sizeof(T) / 16); ++i) {
+                const bool in = col + (i + 1) * static_cast<int>(16 / sizeof(T)) <= a.ffn;
+                reinterpret_cast<uint4 *>(dh)[i] = in ? reinterpret_cast<const uint4 *>(from)[i] : make_uint4(0, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { dh[i] = col + i < a.ffn ? from[i] : from_f32<T>(0.f); }
+        }
+        constexpr int kCols = Saved<T>::kCols;
+        const unsigned char *s = a.saved + r * Saved<T>::row_bytes(a.ffn) + col / kCols * Saved<T>::kBytes;
+        const int at = static_cast<int>(col % kCols);
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                reinterpret_cast<uint4 *>(g)[i] = reinterpret_cast<const uint4 *>(s + 4 * at)[i];
+                reinterpret_cast<uint4 *>(u)[i] = reinterpret_cast<const uint4 *>(s + 64 + 4 * at)[i];
+            }
+        } else {
+            *reinterpret_cast<uint4 *>(g) = *reinterpret_cast<const uint4 *>(s + 2 * at);
+            *reinterpret_cast<uint4 *>(u) = *reinterpret_cast<const uint4 *>(s + 32 + 2 * at);
+            low_g = *reinterpret_cast<const uint2 *>(s + 64 + at);
+            low_u = *reinterpret_cast<const uint2 *>(s + 80 + at);
+        }
+    }
+    __device__ __forceinline__ static float value(const uint32_t *v, const uint2 &low, int i)
+    {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(v[i]);
+        } else {
+            // bytes: 0, the next 8 bits, the upper 16
+            const uint32_t lo = __byte_perm(i < 4 ? low.x : low.y, 0u, 0x4404 | ((i & 3) << 4));
+            return __uint_as_float(__byte_perm(v[i / 2], lo, (i & 1) != 0 ? 0x3254 : 0x1054));
+        }
+    }
 };
 
 template <typename T, int kAct>
@@ -171,56 +334,44 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(GateGrad a)
 {
     __shared__ float sums[2][8][kGradCols];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const long long col = blockIdx.x * static_cast<long long>(kGradCols) + 8 * tx;
-    const long long first = blockIdx.y * static_cast<long long>(kGradRows);
+    const int across = static_cast<int>((a.ffn + kGradCols - 1) / kGradCols), down = blockIdx.x / across;
+    const long long base = (blockIdx.x - down * across) * static_cast<long long>(kGradCols), col = base + 8 * tx;
+    const long long first = down * static_cast<long long>(kGradRows);
+    const long long end = min(first + kGradRows, a.tokens), slab = a.tokens * a.pitch;
     float sg[8] = {}, su[8] = {};
     if (col < a.ffn) {
-        for (long long r = first + ty; r < min(first + kGradRows, a.tokens); r += 8) {
-            float dh[8], g[8], u[8];
-            const T *from = static_cast<const T *>(a.dh) + r * a.dh_row + col;
-            if (a.vec && col + 8 <= a.ffn) {
-                __align__(16) T t[8];
-                for (int i = 0; i < static_cast<int>(8 * sizeof(T) / 16); ++i) {
-                    reinterpret_cast<uint4 *>(t)[i] = reinterpret_cast<const uint4 *>(from)[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) { dh[i] = to_f32(t[i]); }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) { dh[i] = col + i < a.ffn ? to_f32(from[i]) : 0.f; }
-            }
-            const float4 *pg = reinterpret_cast<const float4 *>(a.saved + r * a.pitch + col);
-            const float4 *pu = reinterpret_cast<const float4 *>(a.saved + (a.tokens + r) * a.pitch + col);
-            reinterpret_cast<float4 *>(g)[0] = pg[0];
-            reinterpret_cast<float4 *>(g)[1] = pg[1];
-            reinterpret_cast<float4 *>(u)[0] = pu[0];
-            reinterpret_cast<float4 *>(u)[1] = pu[1];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float dg = dh[i] * u[i] * act_grad<kAct>(g[i]), du = dh[i] * act<kAct>(g[i]);
-                g[i] = dg;
-                u[i] = du;
-                sg[i] += dg;
-                su[i] += du;
-            }
+        GateGradRow<T> row;
+        if (first + ty < end) { row.load(a, first + ty, col); }
+        for (long long r = first + ty; r < end; r += 8) {
+            const GateGradRow<T> now = row;
+            if (r + 8 < end) { row.load(a, r + 8, col); }
             constexpr int kSlabs = sizeof(T) == 4 ? kPieces : 1;
-            const long long slab = a.tokens * a.pitch;
-            uint16_t *at = a.d + r * a.pitch + col;
             __align__(16) uint16_t out[2][kSlabs][8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
+                const float dh = to_f32(now.dh[i]), g = now.value(now.g, now.low_g, i), u = now.value(now.u, now.low_u, i);
+                float act, grad;
+                act_both<T, kAct>(g, act, grad);
+                const float dg = dh * u * grad, du = dh * act;
+                if (col + i < a.ffn) {
+                    sg[i] += dg;
+                    su[i] += du;
+                }
                 if constexpr (sizeof(T) == 4) {
                     uint16_t piece[kPieces];
-                    cut(g[i], piece);
+                    cut(dg, piece);
+#pragma unroll
                     for (int j = 0; j < kPieces; ++j) { out[0][j][i] = piece[j]; }
-                    cut(u[i], piece);
+                    cut(du, piece);
+#pragma unroll
                     for (int j = 0; j < kPieces; ++j) { out[1][j][i] = piece[j]; }
                 } else {
-                    const T x = from_f32<T>(g[i]), y = from_f32<T>(u[i]);
+                    const T x = from_f32<T>(dg), y = from_f32<T>(du);
                     out[0][0][i] = *reinterpret_cast<const uint16_t *>(&x);
                     out[1][0][i] = *reinterpret_cast<const uint16_t *>(&y);
                 }
             }
+            uint16_t *at = a.d + r * a.pitch + col;
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
 #pragma unroll
@@ -237,12 +388,12 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(GateGrad a)
         sums[1][ty][8 * tx + i] = su[i];
     }
     __syncthreads();
-    const long long mine = blockIdx.x * static_cast<long long>(kGradCols) + threadIdx.x;
+    const long long mine = base + threadIdx.x;
     if (mine >= a.ffn) { return; }
     for (int z = 0; z < 2; ++z) {
         float sum = 0;
         for (int i = 0; i < 8; ++i) { sum += sums[z][i][threadIdx.x]; }
-        a.partial[(2ll * blockIdx.y + z) * a.ffn + mine] = sum;
+        a.partial[(2ll * down + z) * a.ffn + mine] = sum;
     }
 }
 
@@ -255,6 +406,64 @@ __global__ void bias_sums_kernel(const float *partial, long long blocks, long lo
     double sum = 0;
     for (long long b = 0; b < blocks; ++b) { sum += partial[(2 * b + blockIdx.y) * ffn + j]; }
     store_any(out, j, dt, static_cast<float>(sum));
+}
+
+// ------------------------------------------------------------ few tokens
+// The weights' way from memory is all that counts: a warp takes a row of both, for all tokens.
+constexpr int kFewTokens = 4;
+
+template <typename T, int kAct, int kTokens, bool kVec>
+__global__ void __launch_bounds__(256) few_kernel(stdmlc_gated a)
+{
+    const long long f = blockIdx.x * 8ll + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (f >= a.ffn) { return; }
+    const T *wg = static_cast<const T *>(a.w_gate) + f * a.w_gate_row, *wu = static_cast<const T *>(a.w_up) + f * a.w_up_row;
+    const T *x = static_cast<const T *>(a.x);
+    float g[kTokens] = {}, u[kTokens] = {};
+    constexpr int kPer = kVec ? 16 / static_cast<int>(sizeof(T)) : 1;
+    struct alignas(kVec ? 16 : sizeof(T)) Vec {
+        T v[kPer];
+    };
+#pragma unroll 4
+    for (long long k = lane * kPer; k < a.hidden; k += 32 * kPer) {
+        const Vec vg = *reinterpret_cast<const Vec *>(wg + k), vu = *reinterpret_cast<const Vec *>(wu + k);
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+            const Vec vx = *reinterpret_cast<const Vec *>(x + t * a.x_row + k);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                g[t] += to_f32(vx.v[i]) * to_f32(vg.v[i]);
+                u[t] += to_f32(vx.v[i]) * to_f32(vu.v[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+        g[t] = warp_sum(g[t]);
+        u[t] = warp_sum(u[t]);
+        if (lane != t) { continue; }
+        if (a.b_gate != nullptr) {
+            g[t] += to_f32(static_cast<const T *>(a.b_gate)[f]);
+            u[t] += to_f32(static_cast<const T *>(a.b_up)[f]);
+        }
+        static_cast<T *>(a.h)[t * a.ffn + f] = from_f32<T>(u[t] * act<T, kAct>(g[t]));
+        if (a.saved != nullptr) {
+            constexpr int kCols = Saved<T>::kCols;
+            unsigned char *s = static_cast<unsigned char *>(a.saved) + t * Saved<T>::row_bytes(a.ffn) + f / kCols * Saved<T>::kBytes;
+            const int at = static_cast<int>(f % kCols);
+            const uint32_t bg = __float_as_uint(g[t]), bu = __float_as_uint(u[t]);
+            if constexpr (sizeof(T) == 4) {
+                reinterpret_cast<uint32_t *>(s)[at] = bg;
+                reinterpret_cast<uint32_t *>(s + 64)[at] = bu;
+            } else {
+                reinterpret_cast<uint16_t *>(s)[at] = static_cast<uint16_t>(bg >> 16);
+                reinterpret_cast<uint16_t *>(s + 32)[at] = static_cast<uint16_t>(bu >> 16);
+                s[64 + at] = static_cast<unsigned char>(bg >> 8);
+                s[80 + at] = static_cast<unsigned char>(bu >> 8);
+            }
+        }
+    }
 }
 
 // ------------------------------------------------------------ host side
@@ -350,11 +559,11 @@ struct Operand {
     }
 };
 
-struct Forward {
+struct Operands {
     Bump work;
     Operand x, w_gate, w_up;
 
-    explicit Forward(const stdmlc_gated *a)
+    explicit Operands(const stdmlc_gated *a)
         : work(a->workspace), x(a->x, a->x_row, a->tokens, a->hidden, a->dt, work),
           w_gate(a->w_gate, a->w_gate_row, a->ffn, a->hidden, a->dt, work),
           w_up(a->w_up, a->w_up_row, a->ffn, a->hidden, a->dt, work)
@@ -363,19 +572,6 @@ struct Forward {
 };
 
 long long row_blocks(const stdmlc_gated *a) { return (a->tokens + kGradRows - 1) / kGradRows; }
-long long saved_pitch(const stdmlc_gated *a) { return up_to(a->ffn, 16); }
-
-struct Backward : Forward {
-    Matrix d;
-    float *partial;
-
-    explicit Backward(const stdmlc_gated *a) : Forward(a)
-    {
-        d = {work.take<uint16_t>(2 * pieces_of(a->dt) * a->tokens * saved_pitch(a)), a->tokens, a->ffn, saved_pitch(a),
-             2 * pieces_of(a->dt)};
-        partial = work.take<float>(2 * row_blocks(a) * a->ffn);
-    }
-};
 
 unsigned int *status_word()
 {
@@ -384,39 +580,145 @@ unsigned int *status_word()
     return static_cast<unsigned int *>(p);
 }
 
-// The pairs of pieces whose products are summed, smallest first.
-constexpr signed char kPairs[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};
-
-template <int kCtas, bool kAcrossA, bool kAcrossB, bool kTwoB, typename Epilogue>
-void launch(Product &p, const Epilogue &epilogue, int dt, long long reduction, cudaStream_t s)
+// Sizes of a product, without its operands.
+Product sizes(long long m, long long n, long long reduction, int halves, int z, bool two_b)
 {
+    Product p{};
+    p.m = static_cast<int>(m);
+    p.n = static_cast<int>(n);
     p.steps = static_cast<int>((reduction + kStepK - 1) / kStepK);
-    p.m_tiles = static_cast<int>((p.m + kTileM * kCtas - 1) / (kTileM * kCtas));
-    const int width = kTwoB ? 128 : kTileN;
-    p.n_tiles = static_cast<int>((p.n + width - 1) / width);
-    const uint32_t type = dt == kF16 ? 0u : 1u;
-    p.kind = (1u << 4) | (type << 7) | (type << 10) | (kAcrossA ? 1u << 15 : 0u) | (kAcrossB ? 1u << 16 : 0u) |
-             (static_cast<uint32_t>(kTileN >> 3) << 17) | (static_cast<uint32_t>(kTileM * kCtas >> 4) << 24);
-    p.status = status_word();
-    const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * p.z;
-    require(tiles < (1ll << 30), "gated_linear: too large");
-    auto kernel = product_kernel<kCtas, kAcrossA, kAcrossB, kTwoB, Epilogue>;
-    constexpr int kSmem = product_smem<kCtas>();
-    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem), "shared memory");
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned int>(std::min<long long>(tiles, sm_count() / kCtas) * kCtas));
-    cfg.blockDim = dim3(kProductThreads);
-    cfg.dynamicSmemBytes = kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute pair[1];
-    pair[0].id = cudaLaunchAttributeClusterDimension;
-    pair[0].val.clusterDim = {static_cast<unsigned int>(kCtas), 1, 1};
-    cfg.attrs = pair;
-    cfg.numAttrs = 1;
-    cuda_ok(cudaLaunchKernelEx(&cfg, kernel, p, epilogue), "gated_linear: launch");
+    p.halves = halves;
+    p.z = z;
+    p.two_b = two_b ? 1 : 0;
+    p.m_tiles = static_cast<int>((m + kTileM * kCtas - 1) / (kTileM * kCtas));
+    p.split = 1;
+    return p;
 }
 
-constexpr int kCtas = 2;
+int columns_of(const Product &p, int width)
+{
+    const int w = p.two_b != 0 ? width / 2 : width;
+    return (p.n + w - 1) / w;
+}
+
+// How wide a launch's tiles are and into how many parts those of each product are cut.  C clusters take units in
+// turn, so the launch lasts for
+//   sum over rounds of C units of the longest of each.
+// A unit lasts for its steps (one of a 256-wide tile takes 0.45 us, which is its way from the L2, and of a 128-wide one
+// 0.75 of that, as its bytes), or for the epilogue of the one before it, which runs beside it; the last epilogue runs alone.  The parts
+// of a tile are written (kWrite steps' time), and read by the last (kRead for each).
+int cut_tiles(Work &w, int clusters, bool wide)
+{
+    constexpr int kCuts[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
+    constexpr double kStart = 1, kEpilogue = 6, kWrite = 4, kRead = 4;
+    double least = 1e30;
+    int best[3] = {256, 1, 1};
+    for (int width : {256, 128}) {
+        if (wide && width == 256) { continue; }
+        const double step = width == 256 ? 1.0 : 0.75, area = width / 256.0;
+        int most[2] = {1, 1};
+        long long tiles[2] = {0, 0}, steps[2] = {0, 0};
+        for (int q = 0; q < w.products; ++q) {
+            const Product &p = w.product[q];
+            tiles[q] = static_cast<long long>(p.m_tiles) * columns_of(p, width) * p.z;
+            steps[q] = static_cast<long long>(p.steps) * p.halves;
+            // (parts of 4 steps at least; memory for at most four parts for each cluster)
+            if (tiles[q] <= 2 * clusters) {
+                most[q] = static_cast<int>(std::clamp<long long>(4ll * clusters / tiles[q], 1, std::max(1ll, steps[q] / 4)));
+            }
+        }
+        for (int s0 : kCuts) {
+            for (int s1 : kCuts) {
+                if (s0 > most[0] || s1 > most[1]) { break; }
+                double main[2] = {0, 0}, after[2] = {0, 0};
+                const int s[2] = {s0, s1};
+                for (int q = 0; q < w.products; ++q) {
+                    main[q] = step * steps[q] * w.pairs / s[q] + kStart;
+                    after[q] = area * (s[q] > 1 || wide ? kWrite + kRead * s[q] + kEpilogue : kEpilogue);
+                }
+                const long long u0 = tiles[0] * s0, u1 = tiles[1] * s1;
+                const long long rounds = (u0 + clusters - 1) / clusters, all = (u0 + u1 + clusters - 1) / clusters;
+                const int mixed = u0 % clusters != 0 && u1 > 0 ? 1 : 0;
+                const double unit[2] = {std::max(main[0], after[0]), std::max(main[1], after[1])};
+                const double cost = (rounds - mixed) * unit[0] + mixed * std::max(unit[0], unit[1]) + (all - rounds) * unit[1] +
+                                    (all > rounds ? after[1] : mixed != 0 ? std::max(after[0], after[1]) : after[0]);
+                if (cost < least) {
+                    least = cost;
+                    best[0] = width;
+                    best[1] = s0;
+                    best[2] = s1;
+                }
+            }
+        }
+    }
+    int parts = 0;
+    w.units = 0;
+    for (int q = 0, tile = 0; q < 2; ++q) {
+        Product &p = w.product[q];
+        p.first_unit = q < w.products ? w.units : 0x7fffffff;
+        if (q >= w.products) { break; }
+        p.n_tiles = columns_of(p, best[0]);
+        p.split = best[1 + q];
+        p.first_tile = tile;
+        p.first_part = parts;
+        const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles * p.z;
+        require(w.units + tiles * p.split < (1ll << 23), "gated_linear: too large");
+        tile += static_cast<int>(tiles);
+        w.units += static_cast<int>(tiles) * p.split;
+        if (p.split > 1) { parts += static_cast<int>(tiles) * p.split; }
+    }
+    w.own_part = parts;
+    return best[0];
+}
+
+long long tiles_of(const Product &p) { return static_cast<long long>(p.m_tiles) * p.n_tiles * p.z; }
+
+// Memory of a launch's own: parts and tickets (null where nothing is split).
+struct Scratch {
+    long long tickets = 0;
+
+    Scratch(Work &w, int clusters, int width, Bump &work)
+    {
+        bool split = false;
+        for (int q = 0; q < w.products; ++q) {
+            tickets += tiles_of(w.product[q]) * kCtas * kEpilogueWarps;
+            split = split || w.product[q].split > 1;
+        }
+        if (!split) { tickets = 0; }
+        w.tickets = work.take<unsigned int>(tickets);
+        w.parts = work.take<float>((w.own_part + (w.pairs > 1 ? clusters : 0)) * (width == 256 ? Shape<256>::kPart : Shape<128>::kPart));
+    }
+    void clear(const Work &w, cudaStream_t s) const
+    {
+        if (tickets > 0) { cuda_ok(cudaMemsetAsync(w.tickets, 0, 4 * tickets, s), "cudaMemsetAsync"); }
+    }
+};
+
+void set_kind(Product &p, int dt, int width)
+{
+    const uint32_t type = dt == kF16 ? 0u : 1u;
+    p.kind = (1u << 4) | (type << 7) | (type << 10) | (p.across_a != 0 ? 1u << 15 : 0u) | (p.across_b != 0 ? 1u << 16 : 0u) |
+             (static_cast<uint32_t>(width >> 3) << 17) | (static_cast<uint32_t>(kTileM * kCtas >> 4) << 24);
+}
+
+template <bool kWide, int kN, typename Epilogue>
+void launch_as(const Work &w, const Epilogue &epilogue, int clusters, cudaStream_t s)
+{
+    auto kernel = product_kernel<kWide, kN, Epilogue>;
+    constexpr int kSmem = Shape<kN>::kSmem;
+    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem), "shared memory");
+    kernel<<<static_cast<unsigned int>(std::min(w.units, clusters) * kCtas), kProductThreads, kSmem, s>>>(w, epilogue);
+}
+
+// (32-bit operands take narrow tiles alone: their sums need the registers)
+template <bool kWide, typename Epilogue>
+void launch(const Work &w, const Epilogue &epilogue, int clusters, int width, cudaStream_t s)
+{
+    if constexpr (!kWide) {
+        if (width == 256) { return launch_as<false, 256>(w, epilogue, clusters, s); }
+    }
+    launch_as<kWide, 128>(w, epilogue, clusters, s);
+}
 
 bool aligned_rows(const void *p, long long row, int dt)
 {
@@ -437,6 +739,10 @@ void check(const stdmlc_gated *a)
 
 CUtensorMapDataType map_type(int dt) { return dt == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
 
+// 32-bit sums of pieces are added up in registers after so many steps: the tensor cores cut what they add to a
+// sum of its size, a step of 2^-24 each time, always towards zero.
+constexpr int kWideChunk = 2;
+
 template <typename F>
 void by_gate(int act, F f)
 {
@@ -453,87 +759,167 @@ void by_gate(int act, F f)
     }
 }
 
+struct Forward : Operands {
+    int clusters = sm_count() / kCtas, width = 0;
+    Work w{};
+    Scratch scratch;
+
+    explicit Forward(const stdmlc_gated *a) : Operands(a), scratch{plan(a), clusters, width, work} {}
+
+  private:
+    Work &plan(const stdmlc_gated *a)
+    {
+        w.product[0] = sizes(a->tokens, a->ffn, a->hidden, 1, 1, true);
+        w.products = 1;
+        w.pairs = a->dt == kF32 ? 6 : 1;
+        w.chunk = kWideChunk;
+        width = cut_tiles(w, clusters, a->dt == kF32);
+        return w;
+    }
+};
+
+struct Backward : Operands {
+    int clusters = sm_count() / kCtas, width = 0, dx = -1, dw = -1;
+    Matrix d;
+    float *partial;
+    Work w{};
+    Scratch scratch;
+
+    explicit Backward(const stdmlc_gated *a) : Operands(a), d(grads(a)), partial(work.take<float>(2 * row_blocks(a) * a->ffn)),
+          scratch{plan(a), clusters, width, work}
+    {
+    }
+
+  private:
+    Matrix grads(const stdmlc_gated *a)
+    {
+        const long long pitch = up_to(a->ffn, 8);
+        return {work.take<uint16_t>(2 * pieces_of(a->dt) * a->tokens * pitch), a->tokens, a->ffn, pitch, 2 * pieces_of(a->dt)};
+    }
+    Work &plan(const stdmlc_gated *a)
+    {
+        const int pieces = pieces_of(a->dt), z = (a->dw_gate != nullptr ? 1 : 0) + (a->dw_up != nullptr ? 1 : 0);
+        Product px = sizes(a->tokens, a->hidden, a->ffn, 2, 1, false), pw = sizes(a->ffn, a->hidden, a->tokens, 1, z, false);
+        px.half_slabs = pieces;
+        px.across_b = 1;
+        pw.z_slabs = pieces;
+        pw.z_first = a->dw_gate != nullptr ? 0 : 1;
+        pw.across_a = pw.across_b = 1;
+        // (the longer units first: they run beside the shorter ones of the other product)
+        const bool x_first = 2 * px.steps >= pw.steps;
+        for (int turn = 0; turn < 2; ++turn) {
+            const bool x = (turn == 0) == x_first;
+            if (x && a->dx != nullptr) { w.product[dx = w.products++] = px; }
+            if (!x && z > 0) { w.product[dw = w.products++] = pw; }
+        }
+        w.pairs = a->dt == kF32 ? 6 : 1;
+        w.chunk = kWideChunk;
+        if (w.products > 0) { width = cut_tiles(w, clusters, a->dt == kF32); }
+        return w;
+    }
+};
+
+template <typename T, int kTokens>
+void few(const stdmlc_gated *a, cudaStream_t s)
+{
+    const bool vec = aligned_rows(a->x, a->tokens > 1 ? a->x_row : 8, a->dt) && aligned_rows(a->w_gate, a->w_gate_row, a->dt) &&
+                     aligned_rows(a->w_up, a->w_up_row, a->dt) && a->hidden * sizeof(T) % 16 == 0;
+    const unsigned int blocks = static_cast<unsigned int>((a->ffn + 7) / 8);
+    by_gate(a->act, [&](auto k) {
+        constexpr int kAct = decltype(k)::value;
+        if (vec) {
+            few_kernel<T, kAct, kTokens, true><<<blocks, 256, 0, s>>>(*a);
+        } else {
+            few_kernel<T, kAct, kTokens, false><<<blocks, 256, 0, s>>>(*a);
+        }
+    });
+}
+
 void forward(const stdmlc_gated *a, cudaStream_t s)
 {
-    const Forward f(a);
+    if (a->tokens <= kFewTokens) {
+        by_dtype(a->dt, [&](auto t) {
+            using T = decltype(t);
+            switch (a->tokens) {
+            case 1:
+                return few<T, 1>(a, s);
+            case 2:
+                return few<T, 2>(a, s);
+            case 3:
+                return few<T, 3>(a, s);
+            default:
+                return few<T, 4>(a, s);
+            }
+        });
+        return;
+    }
+    Forward f(a);
     f.x.pack(s);
     f.w_gate.pack(s);
     f.w_up.pack(s);
-    Product p{};
+    Product &p = f.w.product[0];
     p.a = f.x.as.map(map_type(a->dt), kTileM);
-    p.b[0] = f.w_gate.as.map(map_type(a->dt), 128);
-    p.b[1] = f.w_up.as.map(map_type(a->dt), 128);
-    const bool wide = a->dt == kF32;
-    for (int i = wide ? 0 : 5; i < 6; ++i) { p.segments[p.segment_count++] = {kPairs[i][0], 0, kPairs[i][1]}; }
-    p.m = a->tokens;
-    p.n = a->ffn;
-    p.z = 1;
+    p.b[0] = f.w_gate.as.map(map_type(a->dt), f.width / kCtas);
+    p.b[1] = f.w_up.as.map(map_type(a->dt), f.width / kCtas);
+    set_kind(p, a->dt, f.width);
+    f.w.status = status_word();
+    f.scratch.clear(f.w, s);
     by_dtype(a->dt, [&](auto t) {
         using T = decltype(t);
         by_gate(a->act, [&](auto k) {
-            const GatedTile<T, decltype(k)::value> tile{static_cast<T *>(a->h), static_cast<const T *>(a->b_gate),
-                                                        static_cast<const T *>(a->b_up), static_cast<float *>(a->saved),
-                                                        saved_pitch(a), aligned_rows(a->h, a->ffn, a->dt)};
-            launch<kCtas, false, false, true>(p, tile, a->dt, a->hidden, s);
+            const GatedTile<T, decltype(k)::value> tile{
+                static_cast<T *>(a->h),           static_cast<const T *>(a->b_gate),
+                static_cast<const T *>(a->b_up),  static_cast<unsigned char *>(a->saved),
+                aligned_rows(a->h, a->ffn, a->dt), aligned_rows(a->b_gate, 8, a->dt) && aligned_rows(a->b_up, 8, a->dt)};
+            launch<sizeof(T) == 4>(f.w, tile, f.clusters, f.width, s);
         });
     });
 }
 
 void backward(const stdmlc_gated *a, cudaStream_t s)
 {
-    const Backward b(a);
+    Backward b(a);
     const bool sums = a->db_gate != nullptr || a->db_up != nullptr;
-    const GateGrad gg{a->dh, a->dh_row, static_cast<const float *>(a->saved), a->tokens, a->ffn, b.d.pitch,
+    const GateGrad gg{a->dh, a->dh_row, static_cast<const unsigned char *>(a->saved), a->tokens, a->ffn, b.d.pitch,
                       static_cast<uint16_t *>(const_cast<void *>(b.d.ptr)), sums ? b.partial : nullptr,
-                      aligned_rows(a->dh, a->dh_row, a->dt)};
-    const bool wide = a->dt == kF32;
-    const int pieces = pieces_of(a->dt);
+                      aligned_rows(a->dh, a->dh_row, a->dt) && a->ffn * element_size(a->dt) % 16 == 0};
     const CUtensorMapDataType type = map_type(a->dt);
     by_dtype(a->dt, [&](auto t) {
         using T = decltype(t);
         by_gate(a->act, [&](auto k) {
-            const dim3 grid(static_cast<unsigned int>((a->ffn + kGradCols - 1) / kGradCols), static_cast<unsigned int>(row_blocks(a)));
-            gate_grad_kernel<T, decltype(k)::value><<<grid, 256, 0, s>>>(gg);
+            const long long grid = (a->ffn + kGradCols - 1) / kGradCols * row_blocks(a);
+            gate_grad_kernel<T, decltype(k)::value><<<static_cast<unsigned int>(grid), 256, 0, s>>>(gg);
         });
         if (sums) {
             bias_sums_kernel<<<dim3(static_cast<unsigned int>((a->ffn + 255) / 256), 2), 256, 0, s>>>(
                 b.partial, row_blocks(a), a->ffn, a->db_gate, a->db_up, a->dt);
         }
-        if (a->dx != nullptr) {
+        if (b.w.products == 0) { return; }
+        PlainTile<T> tile{{{nullptr, nullptr}, {nullptr, nullptr}}, true};
+        if (b.dx >= 0) {
             b.w_gate.pack(s);
             b.w_up.pack(s);
-            Product p{};
+            Product &p = b.w.product[b.dx];
             p.a = b.d.map(type, kTileM);
             p.b[0] = b.w_gate.as.map(type, kStepK);
             p.b[1] = b.w_up.as.map(type, kStepK);
-            for (int i = wide ? 0 : 5; i < 6; ++i) {
-                for (int z = 0; z < 2; ++z) {
-                    p.segments[p.segment_count++] = {static_cast<signed char>(z * pieces + kPairs[i][0]),
-                                                     static_cast<signed char>(z), kPairs[i][1]};
-                }
-            }
-            p.m = a->tokens;
-            p.n = a->hidden;
-            p.z = 1;
-            const PlainTile<T> tile{{static_cast<T *>(a->dx), nullptr}, aligned_rows(a->dx, a->hidden, a->dt)};
-            launch<kCtas, false, true, false>(p, tile, a->dt, a->ffn, s);
+            set_kind(p, a->dt, b.width);
+            tile.out[b.dx][0] = static_cast<T *>(a->dx);
+            tile.vec = tile.vec && aligned_rows(a->dx, a->hidden, a->dt);
         }
-        if (a->dw_gate != nullptr || a->dw_up != nullptr) {
+        if (b.dw >= 0) {
             b.x.pack(s);
-            Product p{};
+            Product &p = b.w.product[b.dw];
             p.a = b.d.map(type, kStepK);
-            p.b[0] = p.b[1] = b.x.as.map(type, kStepK);
-            for (int i = wide ? 0 : 5; i < 6; ++i) { p.segments[p.segment_count++] = {kPairs[i][0], 0, kPairs[i][1]}; }
-            p.m = a->ffn;
-            p.n = a->hidden;
-            p.z_slabs = pieces;
-            p.z_first = a->dw_gate != nullptr ? 0 : 1;
-            p.z = a->dw_gate != nullptr && a->dw_up != nullptr ? 2 : 1;
-            const PlainTile<T> tile{{static_cast<T *>(a->dw_gate), static_cast<T *>(a->dw_up)},
-                                    (a->dw_gate == nullptr || aligned_rows(a->dw_gate, a->hidden, a->dt)) &&
-                                        (a->dw_up == nullptr || aligned_rows(a->dw_up, a->hidden, a->dt))};
-            launch<kCtas, true, true, false>(p, tile, a->dt, a->tokens, s);
+            p.b[0] = b.x.as.map(type, kStepK);
+            set_kind(p, a->dt, b.width);
+            tile.out[b.dw][0] = static_cast<T *>(a->dw_gate);
+            tile.out[b.dw][1] = static_cast<T *>(a->dw_up);
+            for (const void *p : {a->dw_gate, a->dw_up}) { tile.vec = tile.vec && (p == nullptr || aligned_rows(p, a->hidden, a->dt)); }
         }
+        b.w.status = status_word();
+        b.scratch.clear(b.w, s);
+        launch<sizeof(T) == 4>(b.w, tile, b.clusters, b.width, s);
     });
 }
 }  // namespace
@@ -543,12 +929,14 @@ using namespace stdml::collective::train;
 
 extern "C" long long stdmlc_gated_saved(const stdmlc_gated *a)
 {
-    return a == nullptr ? -1 : 8 * a->tokens * saved_pitch(a);
+    if (a == nullptr) { return -1; }
+    return a->tokens * (a->dt == kF32 ? Saved<float>::row_bytes(a->ffn) : Saved<__half>::row_bytes(a->ffn));
 }
 
 extern "C" long long stdmlc_gated_workspace(const stdmlc_gated *a, int backward)
 {
-    if (a == nullptr) { return -1; }
+    if (a == nullptr || a->tokens < 0 || a->hidden <= 0 || a->ffn <= 0) { return -1; }
+    if (a->tokens == 0 || (!backward && a->tokens <= kFewTokens)) { return 0; }
     return backward ? Backward(a).work.used() : Forward(a).work.used();
 }
 

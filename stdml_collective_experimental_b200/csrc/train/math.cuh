@@ -50,42 +50,76 @@ __device__ __forceinline__ void store_any(void *p, long long i, int dt, float v)
     }
 }
 
-// Activations and their derivatives.  `Z`: float, or double where a value next to a
-// border is placed.
 constexpr float kSqrtHalf = 0.70710678118654752f;   // 1 / sqrt(2)
 constexpr float kGauss = 0.39894228040143268f;      // 1 / sqrt(2 pi)
 constexpr float kTanhScale = 0.79788456080286536f;  // sqrt(2 / pi)
 constexpr float kTanhCube = 0.044715f;
 
-template <int kAct>
+// The hardware's exponential (base 2) and reciprocal, off by about 2^-22.
+__device__ __forceinline__ float fast_exp2(float v)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float fast_rcp(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+
+// z's activation and the derivative there, for results of type T.  32-bit results take CUDA's functions.  For 16-bit
+// ones the exponential and the quotient are the hardware's, and erfc(x) = poly(1 / (1 + px)) * exp(-x^2)
+// after Abramowitz and Stegun, 7.1.26 (off by 1.5e-7 at most), whose exponential the derivative needs anyway: what
+// is left out lies below 2^-10 of half a step of f16, and the kernels would otherwise spend longer on erf than on memory.
+template <typename T, int kAct>
+__device__ __forceinline__ void act_both(float z, float &a, float &d)
+{
+    constexpr bool kExact = sizeof(T) == 4;
+    if constexpr (kAct == STDMLC_ACT_NONE) {
+        a = z;
+        d = 1.f;
+    } else if constexpr (kAct == STDMLC_ACT_RELU) {
+        a = z > 0.f ? z : (z != z ? z : 0.f);
+        d = z > 0.f ? 1.f : 0.f;
+    } else if constexpr (kAct == STDMLC_ACT_SILU) {
+        const float s = kExact ? 1.f / (1.f + expf(-z)) : fast_rcp(1.f + fast_exp2(-kLog2E * z));
+        a = z * s;
+        d = s + a * (1.f - s);
+    } else if constexpr (kAct == STDMLC_ACT_GELU && kExact) {
+        const float c = 0.5f * (1.f + erff(z * kSqrtHalf));
+        a = z * c;
+        d = c + z * kGauss * expf(-0.5f * z * z);
+    } else if constexpr (kAct == STDMLC_ACT_GELU) {
+        // q = erfc(|z| / sqrt 2) / 2: z (1 - q) right of zero, z q left of it.  (Beyond 30, where q is 0, |z| does not
+        // matter; an infinity would.)
+        const float x = fminf(fabsf(z), 30.f), t = fast_rcp(1.f + 0.3275911f * kSqrtHalf * x), e = fast_exp2(-0.5f * kLog2E * z * z);
+        const float q = e * t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+        a = fmaxf(z, 0.f) - x * q;
+        d = (z < 0.f ? q : 1.f - q) + z * (kGauss * e);
+    } else {
+        // s = (1 + tanh y) / 2, which is 0 or 1 long before |z| = 30
+        const float z2 = fminf(z * z, 900.f), y = kTanhScale * z * (1.f + kTanhCube * z2);
+        const float s = kExact ? 1.f / (1.f + expf(-2.f * y)) : fast_rcp(1.f + fast_exp2(-2.f * kLog2E * y));
+        a = z * s;
+        d = s + 2.f * a * (1.f - s) * kTanhScale * (1.f + 3.f * kTanhCube * z2);
+    }
+}
+template <typename T, int kAct>
 __device__ __forceinline__ float act(float z)
 {
-    if constexpr (kAct == STDMLC_ACT_RELU) { return z > 0.f ? z : (z != z ? z : 0.f); }
-    if constexpr (kAct == STDMLC_ACT_SILU) { return z / (1.f + expf(-z)); }
-    if constexpr (kAct == STDMLC_ACT_GELU) { return 0.5f * z * (1.f + erff(z * kSqrtHalf)); }
-    if constexpr (kAct == STDMLC_ACT_GELU_TANH) {
-        return 0.5f * z * (1.f + tanhf(kTanhScale * (z + kTanhCube * z * z * z)));
-    }
-    return z;
+    float a, d;
+    act_both<T, kAct>(z, a, d);
+    return a;
 }
-
-template <int kAct>
+template <typename T, int kAct>
 __device__ __forceinline__ float act_grad(float z)
 {
-    if constexpr (kAct == STDMLC_ACT_RELU) { return z > 0.f ? 1.f : 0.f; }
-    if constexpr (kAct == STDMLC_ACT_SILU) {
-        const float s = 1.f / (1.f + expf(-z));
-        return s * (1.f + z * (1.f - s));
-    }
-    if constexpr (kAct == STDMLC_ACT_GELU) {
-        return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kGauss * expf(-0.5f * z * z);
-    }
-    if constexpr (kAct == STDMLC_ACT_GELU_TANH) {
-        const float th = tanhf(kTanhScale * (z + kTanhCube * z * z * z));
-        return 0.5f * (1.f + th) +
-               0.5f * z * (1.f - th * th) * kTanhScale * (1.f + 3.f * kTanhCube * z * z);
-    }
-    return 1.f;
+    float a, d;
+    act_both<T, kAct>(z, a, d);
+    return d;
 }
 
 template <typename V>

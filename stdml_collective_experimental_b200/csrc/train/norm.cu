@@ -97,7 +97,7 @@ __global__ void apply_kernel(NormArgs a)
         const double *st = a.stats + 2 * (n * a.groups + c / a.per);
         const float r = a.r.ptr != nullptr ? at<T>(a.r, n, s, c) : 0.f;
         const float z = pre_activation<kAct>(at<T>(a.x, n, s, c), st[0], st[1], weight_of(a, c), bias_of(a, c), r);
-        put<T>(a.y, a.ys, n, s, c, act<kAct>(z));
+        put<T>(a.y, a.ys, n, s, c, act<T, kAct>(z));
     }
 }
 
@@ -108,7 +108,7 @@ __device__ __forceinline__ float grad_z(const NormArgs &a, long long n, long lon
     const float r = a.r.ptr != nullptr ? at<T>(a.r, n, s, c) : 0.f, x = at<T>(a.x, n, s, c);
     const float z = pre_activation<kAct>(x, st[0], st[1], weight_of(a, c), bias_of(a, c), r);
     xh = (x - static_cast<float>(st[0])) * static_cast<float>(st[1]);
-    return at<T>(a.dy, n, s, c) * act_grad<kAct>(z);
+    return at<T>(a.dy, n, s, c) * act_grad<T, kAct>(z);
 }
 
 template <typename T, int kAct>

@@ -1,38 +1,65 @@
 // Matrix products on the tensor cores: a persistent kernel in which one warp brings tiles of the operands
-// into shared memory (TMA), one thread issues the products (tcgen05), and eight warps take finished tiles out of tensor
+// into shared memory (TMA), one thread issues the products (tcgen05), and sixteen warps take finished tiles out of tensor
 // memory and through an epilogue while the next tile is summed.
 //
-// A tile is 128 (kCtas == 1) or 256 (2: a pair of CTAs works on one) by 256, summed in 32 bits.
+// A tile is 256 by kN (256 or 128); a pair of CTAs works on it (each loads its own 128 rows of A and half the columns of
+// B), and it is summed in 32 bits.  What a launch computes is cut into units: a tile, or one of
+// `split` parts of its reduction, where whole tiles would not keep all SMs busy.  Whoever comes last to a tile that was
+// split sums its parts, in their order, so that results do not depend on who that is.
 #pragma once
 #include "math.cuh"
 #include "ptx.cuh"
 
 namespace stdml::collective::train
 {
-constexpr int kTileM = 128;       // rows of a CTA
-constexpr int kTileN = 256;       // columns of a tile
-constexpr int kStepK = 64;        // of the reduction: 128 bytes
-constexpr int kChunk = 128 * 128; // bytes of 128 rows (or columns) by one step
-constexpr int kEpilogueWarps = 8;
+constexpr int kCtas = 2;
+constexpr int kTileM = 128;        // rows of a CTA
+constexpr int kStepK = 64;         // of the reduction: 128 bytes
+constexpr int kChunkA = kTileM * 128;  // bytes of A's 128 rows by one step
+constexpr int kEpilogueWarps = 16;     // (with 8 the epilogue of a gated tile of 12 steps took three times its products)
+constexpr int kSlices = kEpilogueWarps / 4;
 constexpr int kProductThreads = 32 * (4 + kEpilogueWarps);
-constexpr int kMostSegments = 12;
+constexpr int kStagingBytes = 4096;  // of an epilogue warp: 32 rows of 128 bytes
 
-// What a product reads: a sum over segments, each a product over the whole reduction.  A and B are slabs of their maps.
-struct Segment {
-    signed char a_slab, b_map, b_slab;
+// What depends on the width of a tile.
+template <int kN>
+struct Shape {
+    static constexpr int kChunkB = kN / kCtas * 128;
+    static constexpr int kStageBytes = kChunkA + kChunkB;
+    static constexpr int kStages = kN == 256 ? 5 : 6;
+    static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024 /* alignment */ + 256 /* barriers */;
+    static constexpr int kValues = kN / kSlices;  // of a tile that an epilogue thread takes
+    static constexpr int kBlocks = kValues / 16;
+    static constexpr long long kPart = static_cast<long long>(kCtas) * kEpilogueWarps * 32 * kValues;  // values of a part
 };
 
+// A result, or several (z) of one shape, as sums of products over a reduction.  32-bit operands come in pieces, of
+// which `pairs` products are summed.
 struct Product {
     CUtensorMap a, b[2];
-    Segment segments[kMostSegments];
-    int segment_count;
-    int steps;                // of the reduction, per segment
-    long long m, n;           // of the result (n: of each half in a gated tile)
-    int m_tiles, n_tiles, z;  // z results side by side: A's slabs z_slabs apart
-    int z_slabs, z_first;
+    int across_a, across_b;   // the operand's rows lie along the reduction (it runs across them)
+    int two_b;                // half of a tile's columns by b[0], the same columns by b[1] in the other half
+    int steps;                // of the reduction
+    int halves;               // reductions one after the other: A's slabs half_slabs apart, the second with b[1]
+    int half_slabs, z_slabs;  // A's slabs from one half, from one result to the next
+    int m, n;                 // of the result (n: of either half in a tile with two B)
+    int m_tiles, n_tiles, z, z_first;
+    int split, first_unit, first_tile, first_part;
     uint32_t kind;            // instruction descriptor
+};
+
+struct Work {
+    Product product[2];
+    int products, units, pairs;
+    int chunk;          // steps that are summed in tensor memory before 32-bit registers take over (0: all)
+    float *parts;       // kPart values for each unit of a split product, then (kWide) for each cluster, from own_part on
+    int own_part;
+    unsigned int *tickets;  // zero: [tile][CTA of the pair][epilogue warp]
     unsigned int *status;
 };
+
+// The pairs of pieces whose products reach 2^-24 of the largest, smallest first.
+__device__ constexpr signed char kPairA[6] = {0, 2, 1, 0, 1, 0}, kPairB[6] = {2, 0, 1, 1, 0, 0};
 
 // Why a kernel gave up: a wait ran out.
 constexpr unsigned int kWaitRanOut = 1;
@@ -63,57 +90,131 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile
     return bar_try(bar, parity) || wait_slow(bar, parity, dead, status);
 }
 
-struct Tile {
-    long long m, n;
-    int z;
+// What a unit is: a part of a tile of a product.
+struct Unit {
+    int product, tile, part;  // (the tile's number counts all products' tiles)
+    int m, n, z;              // first row, tile column, result
+    int from, to;             // steps of the reduction, over all halves
 };
 
-// Tiles that run at the same time share operands: bands of kBand tile rows, column by column.
-template <int kCtas>
-__device__ __forceinline__ Tile tile_at(const Product &p, int i)
+// n / d for 0 <= n < 2^23 by the quotient in 32-bit floats, which is off by one at most.  (The compiler's division, five in
+// a row, cost each unit 1 us.)
+__device__ __forceinline__ int divided(int n, int d)
 {
-    constexpr int kBand = 16 / kCtas;
-    const int per = p.m_tiles * p.n_tiles, z = i / per;
-    i -= z * per;
-    const int band = i / (kBand * p.n_tiles), first = band * kBand;
-    const int high = min(kBand, p.m_tiles - first);
-    i -= band * kBand * p.n_tiles;
-    return {static_cast<long long>(first + i % high) * (kTileM * kCtas), static_cast<long long>(i / high), z + p.z_first};
+    const int q = __float2int_rz(__fdividef(static_cast<float>(n), static_cast<float>(d)));
+    const int r = n - q * d;
+    return r < 0 ? q - 1 : r >= d ? q + 1 : q;
 }
 
-template <int kCtas>
-constexpr int stages()
+__device__ __forceinline__ Unit unit_at(const Work &w, int i)
 {
-    return kCtas == 2 ? 6 : 4;
-}
-template <int kCtas>
-constexpr int stage_bytes()
-{
-    return kChunk + kChunk * 2 / kCtas;
-}
-template <int kCtas>
-constexpr int product_smem()
-{
-    return stages<kCtas>() * stage_bytes<kCtas>() + 1024 /* alignment */ + 256 /* barriers */;
+    // Tiles that run at the same time share operands: bands of kBand tile rows, column by column.
+    constexpr int kBand = 8;
+    Unit u;
+    u.product = i >= w.product[1].first_unit ? 1 : 0;
+    const Product &p = w.product[u.product];
+    i -= p.first_unit;
+    const int steps = p.steps * p.halves;
+    int tile = i;
+    u.part = 0;
+    u.from = 0;
+    u.to = steps;
+    if (p.split > 1) {  // (steps * split < 2^23 too)
+        tile = divided(i, p.split);
+        u.part = i - tile * p.split;
+        u.from = divided(steps * u.part, p.split);
+        u.to = divided(steps * (u.part + 1), p.split);
+    }
+    u.tile = p.first_tile + tile;
+    const int per = p.m_tiles * p.n_tiles;
+    int z = 0;
+    for (; z + 1 < p.z && tile >= per; ++z) { tile -= per; }
+    const int band = divided(tile, kBand * p.n_tiles), first = band * kBand, high = min(kBand, p.m_tiles - first);
+    const int in_band = tile - first * p.n_tiles;
+    u.n = divided(in_band, high);
+    u.m = (first + in_band - u.n * high) * (kTileM * kCtas);
+    u.z = z + p.z_first;
+    return u;
 }
 
-// kAcrossA, kAcrossB: the operand's rows lie along the reduction (its reduction runs across them).
-// Epilogue: void tile(const Product &, m0 of the CTA, n tile, z, warp 0..7, tensor memory address).
-template <int kCtas, bool kAcrossA, bool kAcrossB, bool kTwoB, typename Epilogue>
-__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Product p,
-                                                                     const __grid_constant__ Epilogue epilogue)
+// Where the 16 values of a block of a thread's lie in a tile's tensor memory: those of a slice side by side, of a
+// gated tile half of them in either half.
+template <int kN>
+__device__ __forceinline__ int block_column(bool two_b, int slice, int block)
+{
+    constexpr int kOf = Shape<kN>::kValues, kHalf = Shape<kN>::kBlocks / 2;
+    return two_b ? kOf / 2 * slice + 16 * (block % kHalf) + block / kHalf * (kN / 2) : kOf * slice + 16 * block;
+}
+
+// The values of a finished tile: in tensor memory, or in parts that are added up.
+template <int kN>
+struct FromTensorMemory {
+    uint32_t at;
+    bool two_b;
+    int slice;
+    __device__ __forceinline__ void load(int block, float (&v)[16]) const
+    {
+        tmem_load16(at + block_column<kN>(two_b, slice, block), v);
+    }
+    __device__ __forceinline__ void loaded(float (&v)[16]) const { tmem_loaded(v); }
+};
+template <int kN>
+struct FromParts {
+    const float *at;  // of the first part, this thread's first value
+    int count;
+    __device__ __forceinline__ void load(int block, float (&v)[16]) const
+    {
+        const float *p = at + block * 16 * 32;
+        int k = 1;
+        if (count > 1) {  // two parts at a time on their way
+            float second[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { v[i] = __ldcg(p + 32 * i); }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { second[i] = __ldcg(p + Shape<kN>::kPart + 32 * i); }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { v[i] += second[i]; }
+            k = 2;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { v[i] = __ldcg(p + 32 * i); }
+        }
+        for (; k < count; k += 2) {
+            float first[16], second[16];
+            const bool two = k + 1 < count;
+            const float *q = p + k * Shape<kN>::kPart;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { first[i] = __ldcg(q + 32 * i); }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { second[i] = two ? __ldcg(q + Shape<kN>::kPart + 32 * i) : 0.f; }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { v[i] = v[i] + first[i] + second[i]; }
+        }
+    }
+    __device__ __forceinline__ void loaded(float (&)[16]) const {}
+};
+
+// kWide: operands in pieces, sums of `chunk` steps added up in registers.  An Epilogue has
+//   template <int kN, typename Source> void tile(const Product &, product, row of the warp's first lane, tile column, z,
+//                                                slice, staging memory of the warp, Source)
+template <bool kWide, int kN, typename Epilogue>
+__global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads, 1)
+    product_kernel(const __grid_constant__ Work w, const __grid_constant__ Epilogue epilogue)
 {
     extern __shared__ unsigned char raw[];
-    constexpr int kStages = stages<kCtas>(), kBytes = stage_bytes<kCtas>(), kChunksB = 2 / kCtas;
     __shared__ uint32_t tmem_at;
     __shared__ int dead_flag;
+    using S = Shape<kN>;
+    constexpr int kStages = S::kStages, kStageBytes = S::kStageBytes;
+    constexpr uint32_t kColumns = 2 * kN;  // of tensor memory: one tile is summed while the other is taken
     unsigned char *ring = raw + ((1024u - (smem_at(raw) & 1023u)) & 1023u);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(ring + kStages * kBytes);
+    unsigned char *staging = ring + kStages * kStageBytes;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * kStagingBytes);
     const uint32_t ring_at = smem_at(ring), full = smem_at(bars), empty = full + 8 * kStages,
                    summed = empty + 8 * kStages, taken = summed + 16;
     volatile int *dead = &dead_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = kCtas == 2 ? cta_rank() : 0u;
+    const uint32_t rank = cta_rank();
 
     if (threadIdx.x == 0) {
         dead_flag = 0;
@@ -127,53 +228,50 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         }
         bar_init_visible();
     }
-    if (warp == 2) { tmem_alloc<kCtas>(smem_at(&tmem_at), 512); }
+    if (warp == 2) { tmem_alloc<kCtas>(smem_at(&tmem_at), kColumns); }
     tmem_before_sync();
     __syncthreads();
-    if constexpr (kCtas == 2) { cluster_sync(); }
+    cluster_sync();
     tmem_after_sync();
     const uint32_t tmem = tmem_at;
-
-    const int tiles = p.m_tiles * p.n_tiles * p.z, workers = gridDim.x / kCtas, first = blockIdx.x / kCtas;
+    const int workers = gridDim.x / kCtas, mine = blockIdx.x / kCtas;
+    const int pairs = kWide ? 6 : 1;
 
     if (warp == 0 && lane == 0) {
         // ---- loads
-        map_prefetch(&p.a);
-        map_prefetch(&p.b[0]);
-        if constexpr (kTwoB) { map_prefetch(&p.b[1]); }
         int it = 0;
         bool ok = true;
-        for (int t = first; ok && t < tiles; t += workers) {
-            const Tile tile = tile_at<kCtas>(p, t);
-            const int m0 = static_cast<int>(tile.m) + static_cast<int>(rank) * kTileM;
-            for (int s = 0; ok && s < p.segment_count; ++s) {
-                const Segment seg = p.segments[s];
-                const int a_slab = seg.a_slab + tile.z * p.z_slabs;
-                for (int k = 0; k < p.steps; ++k, ++it) {
-                    const int st = it % kStages;
-                    ok = it < kStages || wait_for(empty + 8 * st, (it / kStages - 1) & 1, dead, p.status);
-                    if (!ok) { break; }
-                    const uint32_t bar = full + 8 * st, at = ring_at + st * kBytes;
-                    if (rank == 0) { bar_expect(bar, kCtas * kBytes); }
-                    if constexpr (kAcrossA) {
-                        for (int i = 0; i < 2; ++i) {
-                            box_load<kCtas>(at + i * (kChunk / 2), &p.a, m0 + 64 * i, k * kStepK, a_slab, bar);
+        for (int i = mine; ok && i < w.units; i += workers) {
+            const Unit u = unit_at(w, i);
+            const Product &p = w.product[u.product];
+            const int m0 = u.m + static_cast<int>(rank) * kTileM;
+            const int n0 = u.n * (p.two_b ? kN / 2 : kN) + (p.two_b ? 0 : kN / 2 * static_cast<int>(rank));
+            const int chunk = kWide ? w.chunk : u.to - u.from;
+            for (int c = u.from; ok && c < u.to; c += chunk) {
+                for (int pair = 0; ok && pair < pairs; ++pair) {
+                    for (int step = c; step < min(c + chunk, u.to); ++step, ++it) {
+                        const int st = it % kStages;
+                        ok = it < kStages || wait_for(empty + 8 * st, (it / kStages - 1) & 1, dead, w.status);
+                        if (!ok) { break; }
+                        const uint32_t bar = full + 8 * st, at = ring_at + st * kStageBytes;
+                        if (rank == 0) { bar_expect(bar, kCtas * kStageBytes); }
+                        const int second = step >= p.steps ? 1 : 0, k = (step - second * p.steps) * kStepK;
+                        const int a_slab = (kWide ? kPairA[pair] : 0) + second * p.half_slabs + u.z * p.z_slabs;
+                        const int b_slab = kWide ? kPairB[pair] : 0;
+                        const CUtensorMap *b = &p.b[p.two_b ? static_cast<int>(rank) : second];
+                        if (p.across_a) {
+                            box_load<kCtas>(at, &p.a, m0, k, a_slab, bar);
+                            box_load<kCtas>(at + kChunkA / 2, &p.a, m0 + 64, k, a_slab, bar);
+                        } else {
+                            box_load<kCtas>(at, &p.a, k, m0, a_slab, bar);
                         }
-                    } else {
-                        box_load<kCtas>(at, &p.a, k * kStepK, m0, a_slab, bar);
-                    }
+                        if (p.across_b) {
 #pragma unroll
-                    for (int c = 0; c < kChunksB; ++c) {
-                        const int chunk = static_cast<int>(rank) * kChunksB + c;  // of the tile's two
-                        const uint32_t to = at + kChunk * (1 + c);
-                        const CUtensorMap *map = &p.b[kTwoB ? chunk : seg.b_map];
-                        const int n0 = kTwoB ? static_cast<int>(tile.n) * 128 : static_cast<int>(tile.n) * kTileN + 128 * chunk;
-                        if constexpr (kAcrossB) {
-                            for (int i = 0; i < 2; ++i) {
-                                box_load<kCtas>(to + i * (kChunk / 2), map, n0 + 64 * i, k * kStepK, seg.b_slab, bar);
+                            for (int j = 0; j < kN / kCtas; j += 64) {
+                                box_load<kCtas>(at + kChunkA + 128 * j, b, n0 + j, k, b_slab, bar);
                             }
                         } else {
-                            box_load<kCtas>(to, map, k * kStepK, n0, seg.b_slab, bar);
+                            box_load<kCtas>(at + kChunkA, b, k, n0, b_slab, bar);
                         }
                     }
                 }
@@ -181,55 +279,129 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
         }
         // The copies asked for end before the block does: with the products that read them (an arrival on `empty`).
         for (int i = max(0, it - kStages); i < it; ++i) {
-            if (!wait_for(empty + 8 * (i % kStages), (i / kStages) & 1, dead, p.status)) { break; }
+            if (!wait_for(empty + 8 * (i % kStages), (i / kStages) & 1, dead, w.status)) { break; }
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {
         // ---- products
         int it = 0, round = 0;
         bool ok = true;
-        for (int t = first; ok && t < tiles; t += workers, ++round) {
-            const int buf = round & 1;
-            ok = round < 2 || wait_for(taken + 8 * buf, (round / 2 - 1) & 1, dead, p.status);
-            if (!ok) { break; }
-            tmem_after_sync();
-            const uint32_t d = tmem + buf * kTileN;
-            const int steps = p.segment_count * p.steps;
-            for (int k = 0; k < steps; ++k, ++it) {
-                const int st = it % kStages;
-                ok = wait_for(full + 8 * st, (it / kStages) & 1, dead, p.status);
+        for (int i = mine; ok && i < w.units; i += workers) {
+            const Unit u = unit_at(w, i);
+            const Product &p = w.product[u.product];
+            const uint32_t kind = p.kind;
+            const bool across_a = p.across_a != 0, across_b = p.across_b != 0;
+            // 16 further in the reduction: 32 bytes along the rows, or 16 rows
+            const uint64_t next_a = across_a ? 128 : 2, next_b = across_b ? 128 : 2;
+            const int chunk = kWide ? w.chunk : u.to - u.from;
+            for (int c = u.from; ok && c < u.to; c += chunk, ++round) {
+                const int buf = round & 1;
+                ok = round < 2 || wait_for(taken + 8 * buf, (round / 2 - 1) & 1, dead, w.status);
                 if (!ok) { break; }
                 tmem_after_sync();
-                const uint32_t at = ring_at + st * kBytes;
-                const uint64_t a = operand_desc(at, kAcrossA ? kChunk / 2 : 16, 1024);
-                const uint64_t b = operand_desc(at + kChunk, kAcrossB ? kChunk / 2 : 16, 1024);
+                const uint32_t d = tmem + buf * kN;
+                const int steps = (min(c + chunk, u.to) - c) * pairs;
+                for (int k = 0; k < steps; ++k, ++it) {
+                    const int st = it % kStages;
+                    ok = wait_for(full + 8 * st, (it / kStages) & 1, dead, w.status);
+                    if (!ok) { break; }
+                    tmem_after_sync();
+                    const uint32_t at = ring_at + st * kStageBytes;
+                    const uint64_t a = operand_desc(at, across_a ? 64 * 128 : 16, 1024);
+                    const uint64_t b = operand_desc(at + kChunkA, across_b ? 64 * 128 : 16, 1024);
 #pragma unroll
-                for (int j = 0; j < kStepK / 16; ++j) {
-                    // 16 further: 32 bytes along the rows, or 16 rows
-                    mma16<kCtas>(d, a + j * (kAcrossA ? 128 : 2), b + j * (kAcrossB ? 128 : 2), p.kind, k > 0 || j > 0);
+                    for (int j = 0; j < kStepK / 16; ++j) {
+                        mma16<kCtas>(d, a + j * next_a, b + j * next_b, kind, k > 0 || j > 0);
+                    }
+                    mma_commit<kCtas>(empty + 8 * st);
                 }
-                mma_commit<kCtas>(empty + 8 * st);
+                if (ok) { mma_commit<kCtas>(summed + 8 * buf); }
             }
-            if (ok) { mma_commit<kCtas>(summed + 8 * buf); }
         }
     } else if (warp >= 4) {
         // ---- epilogue
+        const int quarter = warp & 3, slice = (warp - 4) >> 2;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+        unsigned char *mem = staging + (warp - 4) * kStagingBytes;
+        const long long place = ((static_cast<long long>(rank) * kEpilogueWarps + (warp - 4)) * S::kValues) * 32 + lane;
         int round = 0;
-        for (int t = first; t < tiles; t += workers, ++round) {
-            const int buf = round & 1;
-            if (!__all_sync(0xffffffffu, wait_for(summed + 8 * buf, (round / 2) & 1, dead, p.status))) { break; }
-            tmem_after_sync();
-            const Tile tile = tile_at<kCtas>(p, t);
-            epilogue.tile(p, tile.m + rank * kTileM, tile.n, tile.z, warp - 4, tmem + buf * kTileN);
-            tmem_before_sync();
-            __syncwarp();
-            if (lane == 0) { bar_arrive_first(taken + 8 * buf); }
+        bool ok = true;
+        for (int i = mine; ok && i < w.units; i += workers) {
+            const Unit u = unit_at(w, i);
+            const Product &p = w.product[u.product];
+            const bool two_b = p.two_b != 0;
+            const int row = u.m + static_cast<int>(rank) * kTileM + 32 * quarter;
+            const long long slot = p.split > 1 ? p.first_part + (i - p.first_unit) : w.own_part + mine;
+            float *part = w.parts + slot * S::kPart + place;
+            if constexpr (kWide) {
+                float sum[S::kValues];
+#pragma unroll
+                for (int j = 0; j < S::kValues; ++j) { sum[j] = 0.f; }
+                for (int c = u.from; c < u.to; c += w.chunk, ++round) {
+                    const int buf = round & 1;
+                    ok = __all_sync(0xffffffffu, wait_for(summed + 8 * buf, (round / 2) & 1, dead, w.status));
+                    if (!ok) { break; }
+                    tmem_after_sync();
+#pragma unroll
+                    for (int b = 0; b < S::kBlocks; ++b) {
+                        float v[16];
+                        tmem_load16(lanes + buf * kN + block_column<kN>(two_b, slice, b), v);
+                        tmem_loaded(v);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) { sum[16 * b + j] += v[j]; }
+                    }
+                    tmem_before_sync();
+                    __syncwarp();
+                    if (lane == 0) { bar_arrive_first(taken + 8 * buf); }
+                }
+                if (!ok) { break; }
+#pragma unroll
+                for (int j = 0; j < S::kValues; ++j) { __stcg(part + 32 * j, sum[j]); }
+            } else {
+                const int buf = round++ & 1;
+                ok = __all_sync(0xffffffffu, wait_for(summed + 8 * buf, ((round - 1) / 2) & 1, dead, w.status));
+                if (!ok) { break; }
+                tmem_after_sync();
+                const uint32_t at = lanes + buf * kN;
+                if (p.split == 1) {
+                    epilogue.template tile<kN>(p, u.product, row, u.n, u.z, slice, mem, FromTensorMemory<kN>{at, two_b, slice});
+                } else {
+#pragma unroll 1
+                    for (int b = 0; b < S::kBlocks; ++b) {
+                        float v[16];
+                        tmem_load16(at + block_column<kN>(two_b, slice, b), v);
+                        tmem_loaded(v);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) { __stcg(part + 32 * (16 * b + j), v[j]); }
+                    }
+                }
+                tmem_before_sync();
+                __syncwarp();
+                if (lane == 0) { bar_arrive_first(taken + 8 * buf); }
+                if (p.split == 1) { continue; }
+            }
+            // This warp's share of the tile: whoever stores the last part adds them up.
+            bool last = true;
+            if (p.split > 1) {
+                __threadfence();
+                __syncwarp();
+                unsigned int before = 0;
+                if (lane == 0) {
+                    before = atomicAdd(w.tickets + (static_cast<long long>(u.tile) * kCtas + rank) * kEpilogueWarps + (warp - 4), 1u);
+                }
+                last = __shfl_sync(0xffffffffu, before, 0) + 1u == static_cast<unsigned int>(p.split);
+                __threadfence();
+            }
+            if (last) {
+                epilogue.template tile<kN>(p, u.product, row, u.n, u.z, slice, mem,
+                                           FromParts<kN>{part - (p.split > 1 ? u.part * S::kPart : 0), p.split});
+            }
         }
     }
     __syncwarp();
     tmem_before_sync();
     __syncthreads();
-    if constexpr (kCtas == 2) { cluster_sync(); }
+    cluster_sync();
     tmem_after_sync();
-    if (warp == 2) { tmem_free<kCtas>(tmem, 512); }
+    if (warp == 2) { tmem_free<kCtas>(tmem, kColumns); }
 }
 }  // namespace stdml::collective::train
