@@ -154,15 +154,17 @@ struct GatedTile {
         const long long first = nt * (kN / 2ll) + kPasses * kCols * slice;
         const RowsOut<kPieces> rows_h(h + first, p.n * static_cast<long long>(sizeof(T)), row0, p.m);
         const RowsOut<kPieces> rows_s(saved + first / kCols * Saved<T>::kBytes, Saved<T>::row_bytes(p.n), row0, p.m);
+        const int passes = static_cast<int>(min(static_cast<long long>(kPasses), (p.n - first + kCols - 1) / kCols));
+        if (passes <= 0) { from.done(); }
 #pragma unroll 1
-        for (int b = 0; b < kPasses; ++b) {
+        for (int b = 0; b < passes; ++b) {
             const long long col = first + kCols * b;
-            if (col >= p.n) { break; }
             float g[16], u[16];
             from.load(b, g);
             from.load(kPasses + b, u);
             from.loaded(g);
             from.loaded(u);
+            if (b == passes - 1) { from.done(); }
             if (b_gate != nullptr) {
                 add_bias(b_gate, col, p.n, g);
                 add_bias(b_up, col, p.n, u);
@@ -205,29 +207,29 @@ struct PlainTile {
     __device__ __forceinline__ void tile(const Product &p, int product, int row0, int nt, int z, int slice, unsigned char *mem,
                                          const Source &from) const
     {
-        constexpr int kOf = Shape<kN>::kValues, kCols = kOf * sizeof(T) > 128 ? 128 / sizeof(T) : kOf;
+        constexpr int kCols = Shape<kN>::kValues, kBytes = kCols * static_cast<int>(sizeof(T));
+        static_assert(kBytes <= 128, "one row in shared memory");
         T *to = product == 0 ? (z == 0 ? out[0][0] : out[0][1]) : (z == 0 ? out[1][0] : out[1][1]);
-        const long long first = nt * static_cast<long long>(kN) + kOf * slice;
-        const RowsOut<kCols * static_cast<int>(sizeof(T)) / 16> rows(to + first, p.n * static_cast<long long>(sizeof(T)), row0, p.m);
-#pragma unroll 1
-        for (int c = 0; c < kOf; c += kCols) {
-            const long long col = first + c;
-            if (col >= p.n) { break; }
-#pragma unroll
-            for (int b = 0; b < kCols / 16; ++b) {
-                float v[16];
-                from.load(c / 16 + b, v);
-                from.loaded(v);
-                put16<T>(mem, threadIdx.x & 31, b * static_cast<int>(sizeof(T)), v);
-            }
-            __syncwarp();
-            if (vec && col + kCols <= p.n) {
-                rows.copy(mem, 0, c * static_cast<int>(sizeof(T)));
-            } else {
-                rows_out_any<T, kCols * sizeof(T)>(mem, to, row0, p.m, p.n, col);
-            }
-            __syncwarp();
+        const long long first = nt * static_cast<long long>(kN) + kCols * slice;
+        if (first >= p.n) {
+            from.done();
+            return;
         }
+#pragma unroll
+        for (int b = 0; b < kCols / 16; ++b) {
+            float v[16];
+            from.load(b, v);
+            from.loaded(v);
+            put16<T>(mem, threadIdx.x & 31, b * static_cast<int>(sizeof(T)), v);
+        }
+        from.done();
+        __syncwarp();
+        if (vec && first + kCols <= p.n) {
+            RowsOut<kBytes / 16>(to + first, p.n * static_cast<long long>(sizeof(T)), row0, p.m).copy(mem, 0, 0);
+        } else {
+            rows_out_any<T, kBytes>(mem, to, row0, p.m, p.n, first);
+        }
+        __syncwarp();
     }
 };
 

@@ -152,11 +152,19 @@ struct FromTensorMemory {
     uint32_t at;
     bool two_b;
     int slice;
+    uint32_t taken;
     __device__ __forceinline__ void load(int block, float (&v)[16]) const
     {
         tmem_load16(at + block_column<kN>(two_b, slice, block), v);
     }
     __device__ __forceinline__ void loaded(float (&v)[16]) const { tmem_loaded(v); }
+    // The warp has all that it wanted: the memory is free for another tile.
+    __device__ __forceinline__ void done() const
+    {
+        tmem_before_sync();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) { bar_arrive_first(taken); }
+    }
 };
 template <int kN>
 struct FromParts {
@@ -192,11 +200,13 @@ struct FromParts {
         }
     }
     __device__ __forceinline__ void loaded(float (&)[16]) const {}
+    __device__ __forceinline__ void done() const {}
 };
 
 // kWide: operands in pieces, sums of `chunk` steps added up in registers.  An Epilogue has
 //   template <int kN, typename Source> void tile(const Product &, product, row of the warp's first lane, tile column, z,
 //                                                slice, staging memory of the warp, Source)
+// which calls the source's done() once, after its last load.
 template <bool kWide, int kN, typename Epilogue>
 __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads, 1)
     product_kernel(const __grid_constant__ Work w, const __grid_constant__ Epilogue epilogue)
@@ -361,23 +371,20 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
                 ok = __all_sync(0xffffffffu, wait_for(summed + 8 * buf, ((round - 1) / 2) & 1, dead, w.status));
                 if (!ok) { break; }
                 tmem_after_sync();
-                const uint32_t at = lanes + buf * kN;
+                const FromTensorMemory<kN> from{lanes + buf * kN, two_b, slice, taken + 8 * buf};
                 if (p.split == 1) {
-                    epilogue.template tile<kN>(p, u.product, row, u.n, u.z, slice, mem, FromTensorMemory<kN>{at, two_b, slice});
-                } else {
-#pragma unroll 1
-                    for (int b = 0; b < S::kBlocks; ++b) {
-                        float v[16];
-                        tmem_load16(at + block_column<kN>(two_b, slice, b), v);
-                        tmem_loaded(v);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) { __stcg(part + 32 * (16 * b + j), v[j]); }
-                    }
+                    epilogue.template tile<kN>(p, u.product, row, u.n, u.z, slice, mem, from);
+                    continue;
                 }
-                tmem_before_sync();
-                __syncwarp();
-                if (lane == 0) { bar_arrive_first(taken + 8 * buf); }
-                if (p.split == 1) { continue; }
+#pragma unroll 1
+                for (int b = 0; b < S::kBlocks; ++b) {
+                    float v[16];
+                    from.load(b, v);
+                    from.loaded(v);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) { __stcg(part + 32 * (16 * b + j), v[j]); }
+                }
+                from.done();
             }
             // This warp's share of the tile: whoever stores the last part adds them up.
             bool last = true;
