@@ -130,6 +130,7 @@ def _declare(l):
     l.stdmlc_dw_check.argtypes = [vp]
     l.stdmlc_dw_recover.argtypes = [vp]
     l.stdmlc_dw_barrier_rows.argtypes = [vp, c.c_int, vp]
+    l.stdmlc_train_status.argtypes = [c.c_int, c.POINTER(c.c_int)]
     l.stdmlc_version.restype = c.c_char_p
     l.stdmlc_dtype_size.argtypes = [c.c_int]
     l.stdmlc_reduce_many.argtypes = [vp, vpp, u64, u64, c.c_int, c.c_int, c.c_double]

@@ -1,6 +1,8 @@
 // The way from an operator on tensors (ops/train.py) to the C ABI: checks of the
 // arguments, layouts that the kernels take, results and workspaces from PyTorch's
-// allocator, the current stream of the tensors' GPU.  What is wrong with the arguments raises
+// allocator, the current stream of the tensors' GPU, and the gradients.  All of it native, the backward pass too,
+// which autograd calls from threads of its own: through Python's Function a training step of small
+// tensors took 85 us, five times what the GPU works.  What is wrong with the arguments raises
 // ValueError / TypeError, before anything is launched; sizes and types are
 // looked at before the place of the data, so that they are refused on any machine.
 #include "train.hpp"
@@ -8,10 +10,12 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <optional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "capi_cuda.h"
@@ -20,56 +24,17 @@
 namespace
 {
 using at::Tensor;
-using Maybe = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::tensor_list;
 
-struct Raised {
-};  // a Python exception is set
+[[noreturn]] void refuse(const char *call, const std::string &what) { TORCH_CHECK_VALUE(false, call, ": ", what); }
+[[noreturn]] void refuse_type(const char *call, const std::string &what) { TORCH_CHECK_TYPE(false, call, ": ", what); }
 
-[[noreturn]] void refuse(const char *call, const std::string &what, PyObject *kind = PyExc_ValueError)
+// Second derivatives would silently lack what goes through the operator.
+void first_order(const char *call)
 {
-    PyErr_SetString(kind, (std::string(call) + ": " + what).c_str());
-    throw Raised{};
+    TORCH_CHECK(!at::GradMode::is_enabled(), call, " is differentiable once: backward with create_graph=True is refused");
 }
-
-struct Args {
-    const char *call;
-    PyObject *const *a;
-    Py_ssize_t n;
-    int i = 0;
-
-    void expect(Py_ssize_t want) const
-    {
-        if (n != want) { refuse(call, std::to_string(want) + " arguments expected", PyExc_TypeError); }
-    }
-    Maybe maybe()
-    {
-        PyObject *o = a[i++];
-        if (o == Py_None) { return {}; }
-        if (!THPVariable_Check(o)) {
-            refuse(call, std::string("tensor expected, got ") + Py_TYPE(o)->tp_name, PyExc_TypeError);
-        }
-        return THPVariable_Unpack(o);
-    }
-    Tensor tensor()
-    {
-        Maybe t = maybe();
-        if (!t) { refuse(call, "tensor expected, got None", PyExc_TypeError); }
-        return *t;
-    }
-    long long integer()
-    {
-        const long long v = PyLong_AsLongLong(a[i++]);
-        if (v == -1 && PyErr_Occurred()) { throw Raised{}; }
-        return v;
-    }
-    bool truth() { return PyObject_IsTrue(a[i++]) == 1; }
-    double real()
-    {
-        const double v = PyFloat_AsDouble(a[i++]);
-        if (v == -1.0 && PyErr_Occurred()) { throw Raised{}; }
-        return v;
-    }
-};
 
 int float_code(const Tensor &t, const char *call)
 {
@@ -81,8 +46,7 @@ int float_code(const Tensor &t, const char *call)
     case c10::ScalarType::Float:
         return 10;
     default:
-        refuse(call, std::string("bfloat16, float16 or float32 expected, got ") + c10::toString(t.scalar_type()),
-               PyExc_TypeError);
+        refuse_type(call, std::string("bfloat16, float16 or float32 expected, got ") + c10::toString(t.scalar_type()));
     }
 }
 
@@ -97,7 +61,7 @@ std::string shape_of(const Tensor &t)
 class OnDevice
 {
   public:
-    OnDevice(const char *call, const Tensor &first, std::initializer_list<const Maybe *> others)
+    OnDevice(const char *call, const Tensor &first, std::initializer_list<const Tensor *> others)
         : device_(checked(call, first, others)), guard_(device_),
           stream_(c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getStream(device_).native_handle())
     {
@@ -106,11 +70,11 @@ class OnDevice
     void *stream() const { return stream_; }
 
   private:
-    static c10::Device checked(const char *call, const Tensor &first, std::initializer_list<const Maybe *> others)
+    static c10::Device checked(const char *call, const Tensor &first, std::initializer_list<const Tensor *> others)
     {
         if (!first.is_cuda()) { refuse(call, "CUDA tensor expected"); }
-        for (const Maybe *t : others) {
-            if (*t && (*t)->device() != first.device()) { refuse(call, "all tensors must lie on one GPU"); }
+        for (const Tensor *t : others) {
+            if (t->defined() && t->device() != first.device()) { refuse(call, "all tensors must lie on one GPU"); }
         }
         return first.device();
     }
@@ -123,44 +87,8 @@ class OnDevice
 void done(int rc)
 {
     if (rc == STDMLC_OK) { return; }
-    PyErr_SetString(rc == STDMLC_ERR_ARGS ? PyExc_ValueError : PyExc_RuntimeError, stdmlc_last_error());
-    throw Raised{};
-}
-
-#define WITHOUT_GIL(rc, call)                                                  \
-    do {                                                                       \
-        Py_BEGIN_ALLOW_THREADS rc = (call);                                    \
-        Py_END_ALLOW_THREADS                                                   \
-    } while (0)
-
-template <typename F>
-PyObject *guarded(F f)
-{
-    try {
-        return f();
-    } catch (const Raised &) {
-        return nullptr;
-    } catch (const std::exception &e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
-    }
-}
-
-PyObject *tuple_of(std::initializer_list<Maybe> all)
-{
-    PyObject *t = PyTuple_New(static_cast<Py_ssize_t>(all.size()));
-    if (t == nullptr) { throw Raised{}; }
-    Py_ssize_t i = 0;
-    for (const Maybe &m : all) {
-        PyObject *o = Py_None;
-        if (m) {
-            o = THPVariable_Wrap(*m);
-        } else {
-            Py_INCREF(o);
-        }
-        PyTuple_SET_ITEM(t, i++, o);
-    }
-    return t;
+    if (rc == STDMLC_ERR_ARGS) { TORCH_CHECK_VALUE(false, stdmlc_last_error()); }
+    TORCH_CHECK(false, stdmlc_last_error());
 }
 
 Tensor bytes_like(const Tensor &t, long long n)
@@ -168,7 +96,21 @@ Tensor bytes_like(const Tensor &t, long long n)
     return at::empty({n}, t.options().dtype(at::kByte).requires_grad(false).memory_format(std::nullopt));
 }
 
-void *ptr_of(const Maybe &t) { return t ? t->data_ptr() : nullptr; }
+void *ptr_of(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// Operands that a call may lack: autograd's Function knows them as empty optionals, the code here as undefined tensors.
+using Maybe = std::optional<Tensor>;
+Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
+Tensor given(const Maybe &t) { return t ? *t : Tensor(); }
+
+bool wanted(std::initializer_list<const Tensor *> all)
+{
+    if (!at::GradMode::is_enabled()) { return false; }
+    for (const Tensor *t : all) {
+        if (t->defined() && t->requires_grad()) { return true; }
+    }
+    return false;
+}
 
 // ------------------------------------------------------------ group normalisation
 // (N, C, spatial...) as rows of channels: the channels side by side, all positions of an image
@@ -218,10 +160,9 @@ Tensor in_rows(const Tensor &t, stdmlc_rows *r)
 struct Norm {
     static constexpr const char *kCall = "group_norm";
     stdmlc_norm a{};
-    Tensor x;
-    Maybe residual, weight, bias;
+    Tensor x, residual, weight, bias;
 
-    void take(const Tensor &x_, const Maybe &residual_, const Maybe &weight_, const Maybe &bias_, long long groups,
+    void take(const Tensor &x_, const Tensor &residual_, const Tensor &weight_, const Tensor &bias_, long long groups,
               double eps, int act)
     {
         x = x_;
@@ -233,23 +174,21 @@ struct Norm {
         if (!(eps >= 0)) { refuse(kCall, "eps must not be negative"); }
         a.dt = float_code(x, kCall);
         a.weight_dt = 10;
-        for (const Maybe *p : {&weight_, &bias_}) {
-            if (!*p) { continue; }
-            if ((*p)->dim() != 1 || (*p)->size(0) != c) {
-                refuse(kCall, "weight and bias of " + std::to_string(c) + " channels expected, got " + shape_of(**p));
+        for (const Tensor *p : {&weight_, &bias_}) {
+            if (!p->defined()) { continue; }
+            if (p->dim() != 1 || p->size(0) != c) {
+                refuse(kCall, "weight and bias of " + std::to_string(c) + " channels expected, got " + shape_of(*p));
             }
-            a.weight_dt = float_code(**p, kCall);
+            a.weight_dt = float_code(*p, kCall);
         }
-        if (weight_ && bias_ && weight_->scalar_type() != bias_->scalar_type()) {
-            refuse(kCall, "weight and bias must have one dtype", PyExc_TypeError);
+        if (weight_.defined() && bias_.defined() && weight_.scalar_type() != bias_.scalar_type()) {
+            refuse_type(kCall, "weight and bias must have one dtype");
         }
-        if (residual_) {
-            if (residual_->sizes() != x.sizes()) {
-                refuse(kCall, "residual of " + shape_of(x) + " expected, got " + shape_of(*residual_));
+        if (residual_.defined()) {
+            if (residual_.sizes() != x.sizes()) {
+                refuse(kCall, "residual of " + shape_of(x) + " expected, got " + shape_of(residual_));
             }
-            if (residual_->scalar_type() != x.scalar_type()) {
-                refuse(kCall, "residual must have the input's dtype", PyExc_TypeError);
-            }
+            if (residual_.scalar_type() != x.scalar_type()) { refuse_type(kCall, "residual must have the input's dtype"); }
         }
         residual = residual_;
         weight = weight_;
@@ -265,84 +204,77 @@ struct Norm {
     void lay_out()
     {
         x = in_rows(x, &a.x);
-        if (residual) { residual = in_rows(*residual, &a.residual); }
-        for (Maybe *p : {&weight, &bias}) {
-            if (*p) { *p = (*p)->contiguous(); }
+        if (residual.defined()) { residual = in_rows(residual, &a.residual); }
+        for (Tensor *p : {&weight, &bias}) {
+            if (p->defined()) { *p = p->contiguous(); }
         }
         a.weight = ptr_of(weight);
         a.bias = ptr_of(bias);
     }
+    // y and the statistics
+    std::pair<Tensor, Tensor> forward()
+    {
+        const OnDevice on(kCall, x, {&residual, &weight, &bias});
+        lay_out();
+        Tensor y = empty_rows(x);
+        Tensor stats = at::empty({a.images, a.groups, 2}, x.options().dtype(at::kDouble).requires_grad(false));
+        rows_of(y, &a.y);
+        a.stats = stats.data_ptr<double>();
+        const Tensor work = bytes_like(x, stdmlc_norm_workspace(&a, 0));
+        a.workspace = work.data_ptr();
+        done(stdmlc_norm_forward(&a, on.index(), on.stream()));
+        return {y, stats};
+    }
 };
 
-// (x, residual | None, weight | None, bias | None, groups, eps, activation) ->
-// (y, statistics, x and residual as the kernels read them)
-PyObject *norm_forward(PyObject *, PyObject *const *args, Py_ssize_t n)
-{
-    return guarded([&] {
-        Args g{Norm::kCall, args, n};
-        g.expect(7);
+struct NormFunction : torch::autograd::Function<NormFunction> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Maybe &residual_, const Maybe &weight_, const Maybe &bias_,
+                          int64_t groups, double eps, int64_t act)
+    {
+        const Tensor residual = given(residual_), weight = given(weight_), bias = given(bias_);
         Norm op;
-        const Tensor x = g.tensor();
-        const Maybe residual = g.maybe(), weight = g.maybe(), bias = g.maybe();
-        const long long groups = g.integer();
-        const double eps = g.real();
-        op.take(x, residual, weight, bias, groups, eps, static_cast<int>(g.integer()));
-        const OnDevice on(Norm::kCall, x, {&residual, &weight, &bias});
-        op.lay_out();
-        Tensor y = empty_rows(x);
-        Tensor stats = at::empty({op.a.images, groups, 2}, x.options().dtype(at::kDouble).requires_grad(false));
-        rows_of(y, &op.a.y);
-        op.a.stats = stats.data_ptr<double>();
-        Tensor work = bytes_like(x, stdmlc_norm_workspace(&op.a, 0));
-        op.a.workspace = work.data_ptr();
-        int rc;
-        WITHOUT_GIL(rc, stdmlc_norm_forward(&op.a, on.index(), on.stream()));
-        done(rc);
-        return tuple_of({y, stats, op.x, op.residual});
-    });
-}
-
-// (dy, x, residual | None, weight | None, bias | None, statistics, groups, eps, activation,
-// want dx, want dresidual, want dweight, want dbias) -> (dx, dresidual, dweight, dbias), None where not wanted
-PyObject *norm_backward(PyObject *, PyObject *const *args, Py_ssize_t n)
-{
-    return guarded([&] {
-        Args g{Norm::kCall, args, n};
-        g.expect(13);
+        op.take(x, residual, weight, bias, groups, eps, static_cast<int>(act));
+        const auto [y, stats] = op.forward();
+        // (x and the residual as the kernels read them; without an activation the residual does not matter)
+        ctx->save_for_backward({op.x, act != STDMLC_ACT_NONE ? op.residual : Tensor(), weight, bias, stats});
+        ctx->saved_data["residual"] = residual.defined();
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["act"] = act;
+        return y;
+    }
+    static tensor_list backward(AutogradContext *ctx, tensor_list grads)
+    {
+        first_order(Norm::kCall);
+        const auto saved = ctx->get_saved_variables();
         Norm op;
-        Tensor dy = g.tensor();
-        const Tensor x = g.tensor();
-        const Maybe residual = g.maybe(), weight = g.maybe(), bias = g.maybe();
-        Tensor stats = g.tensor();
-        const long long groups = g.integer();
-        const double eps = g.real();
-        op.take(x, residual, weight, bias, groups, eps, static_cast<int>(g.integer()));
-        const Maybe dy_ = dy, stats_ = stats;
-        const OnDevice on(Norm::kCall, x, {&residual, &weight, &bias, &dy_, &stats_});
+        const Tensor &weight = saved[2], &bias = saved[3], &stats = saved[4];
+        op.take(saved[0], saved[1], weight, bias, ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(),
+                static_cast<int>(ctx->saved_data["act"].toInt()));
+        const OnDevice on(Norm::kCall, op.x, {&grads[0]});
         op.lay_out();
-        dy = in_rows(dy, &op.a.dy);
+        const Tensor dy = in_rows(grads[0], &op.a.dy);
         op.a.stats = stats.data_ptr<double>();
-        Maybe dx, dres, dw, db;
-        if (g.truth()) {
-            dx = empty_rows(x);
-            rows_of(*dx, &op.a.dx);
+        Tensor dx, dres, dw, db;
+        size_t edge = 0;  // (autograd counts the operands that there are)
+        if (ctx->needs_input_grad(edge++)) {
+            dx = empty_rows(op.x);
+            rows_of(dx, &op.a.dx);
         }
-        if (g.truth()) {
-            dres = empty_rows(x);
-            rows_of(*dres, &op.a.dresidual);
+        if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(edge++)) {
+            dres = empty_rows(op.x);
+            rows_of(dres, &op.a.dresidual);
         }
-        if (g.truth()) { dw = at::empty_like(*op.weight); }
-        if (g.truth()) { db = at::empty_like(*op.bias); }
+        if (weight.defined() && ctx->needs_input_grad(edge++)) { dw = at::empty_like(op.weight); }
+        if (bias.defined() && ctx->needs_input_grad(edge++)) { db = at::empty_like(op.bias); }
         op.a.dweight = ptr_of(dw);
         op.a.dbias = ptr_of(db);
-        Tensor work = bytes_like(x, stdmlc_norm_workspace(&op.a, 1));
+        const Tensor work = bytes_like(op.x, stdmlc_norm_workspace(&op.a, 1));
         op.a.workspace = work.data_ptr();
-        int rc;
-        WITHOUT_GIL(rc, stdmlc_norm_backward(&op.a, on.index(), on.stream()));
-        done(rc);
-        return tuple_of({dx, dres, dw, db});
-    });
-}
+        done(stdmlc_norm_backward(&op.a, on.index(), on.stream()));
+        return {dx, dres, dw, db, {}, {}, {}};
+    }
+};
 
 // ------------------------------------------------------------ rows of a matrix
 // (..., n) as rows with a stride, copied where it does not lie like that.
@@ -382,10 +314,9 @@ bool same_rows(const Tensor &a, const Tensor &b)
 struct Distill {
     static constexpr const char *kCall = "distill_loss";
     stdmlc_distill d{};
-    Tensor logits, top, index;
-    Maybe labels;
+    Tensor logits, top, index, labels;
 
-    void take(const Tensor &logits_, const Tensor &top_, const Tensor &index_, const Maybe &labels_, double temperature,
+    void take(const Tensor &logits_, const Tensor &top_, const Tensor &index_, const Tensor &labels_, double temperature,
               double alpha, long long ignore, int reduction)
     {
         logits = logits_;
@@ -404,14 +335,14 @@ struct Distill {
             refuse(kCall, "teacher_index of " + shape_of(top) + " expected, got " + shape_of(index));
         }
         if (index.scalar_type() != at::kLong && index.scalar_type() != at::kInt) {
-            refuse(kCall, "teacher_index must be int32 or int64", PyExc_TypeError);
+            refuse_type(kCall, "teacher_index must be int32 or int64");
         }
-        if (labels) {
-            if (labels->sizes() != logits.sizes().slice(0, logits.dim() - 1)) {
-                refuse(kCall, "one label for each row expected, got " + shape_of(*labels) + " for " + shape_of(logits));
+        if (labels.defined()) {
+            if (labels.sizes() != logits.sizes().slice(0, logits.dim() - 1)) {
+                refuse(kCall, "one label for each row expected, got " + shape_of(labels) + " for " + shape_of(logits));
             }
-            if (labels->scalar_type() != at::kLong && labels->scalar_type() != at::kInt) {
-                refuse(kCall, "labels must be int32 or int64", PyExc_TypeError);
+            if (labels.scalar_type() != at::kLong && labels.scalar_type() != at::kInt) {
+                refuse_type(kCall, "labels must be int32 or int64");
             }
         }
         if (!(temperature > 0) || !(temperature < 1e30)) { refuse(kCall, "temperature must be positive"); }
@@ -432,81 +363,100 @@ struct Distill {
         top = matrix_of(top, &d.top, &d.top_row);
         index = matrix_of(index, &d.index, &d.index_row);
         d.index_bytes = index.scalar_type() == at::kLong ? 8 : 4;
-        if (labels) {
-            labels = labels->to(at::kLong).contiguous();
-            d.labels = labels->data_ptr();
+        if (labels.defined()) {
+            labels = labels.to(at::kLong).contiguous();
+            d.labels = labels.data_ptr();
         }
     }
+    Tensor empty_grad() const
+    {
+        return at::empty(logits.sizes(), logits.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    }
+    // The loss and the rows' statistics; `grad`: where the gradient goes that the forward pass writes.
+    std::pair<Tensor, Tensor> forward(bool with_grad, Tensor &grad)
+    {
+        const OnDevice on(kCall, logits, {&top, &index, &labels});
+        const auto rows = logits.sizes().slice(0, logits.dim() - 1);
+        lay_out();
+        const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false).memory_format(std::nullopt);
+        Tensor stats = at::empty({d.rows, 5}, f32);
+        Tensor loss = d.reduction == 0 ? at::empty(rows, f32) : at::empty({}, f32);
+        d.row_stats = stats.data_ptr<float>();
+        d.loss = loss.data_ptr<float>();
+        // 16-bit numbers of a small exponent wait for what multiplies them: a loss scale saves them from nothing
+        // once they are rounded
+        if (with_grad && d.reduction != 0 && d.dt != 9) {
+            grad = empty_grad();
+            d.dlogits = grad.data_ptr();
+        }
+        const Tensor work = bytes_like(logits, stdmlc_distill_workspace(&d));
+        d.workspace = work.data_ptr();
+        done(stdmlc_distill_forward(&d, on.index(), on.stream()));
+        captured = stdmlc_stream_capturing(on.stream()) != 0;
+        return {loss, stats};
+    }
+    bool captured = false;
 };
 
-// (logits, teacher_logits, teacher_index, labels | None, temperature, alpha, ignore_index, reduction) ->
-// (loss, row statistics)
-PyObject *distill_forward(PyObject *, PyObject *const *args, Py_ssize_t n)
-{
-    return guarded([&] {
-        Args g{Distill::kCall, args, n};
-        g.expect(8);
+struct DistillFunction : torch::autograd::Function<DistillFunction> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &logits, const Tensor &top, const Tensor &index, const Maybe &labels_,
+                          double temperature, double alpha, int64_t ignore, int64_t reduction)
+    {
+        const Tensor labels = given(labels_);
         Distill op;
-        const Tensor logits = g.tensor(), top = g.tensor(), index = g.tensor();
-        const Maybe labels = g.maybe(), top_ = top, index_ = index;
-        const double temperature = g.real(), alpha = g.real();
-        const long long ignore = g.integer();
-        op.take(logits, top, index, labels, temperature, alpha, ignore, static_cast<int>(g.integer()));
-        const OnDevice on(Distill::kCall, logits, {&top_, &index_, &labels});
-        op.lay_out();
-        const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
-        Tensor stats = at::empty({op.d.rows, 4}, f32);
-        Tensor loss = op.d.reduction == 0 ? at::empty(logits.sizes().slice(0, logits.dim() - 1), f32) : at::empty({}, f32);
-        op.d.row_stats = stats.data_ptr<float>();
-        op.d.loss = loss.data_ptr<float>();
-        Tensor work = bytes_like(logits, stdmlc_distill_workspace(&op.d));
-        op.d.workspace = work.data_ptr();
-        int rc;
-        WITHOUT_GIL(rc, stdmlc_distill_forward(&op.d, on.index(), on.stream()));
-        done(rc);
-        return tuple_of({loss, stats});
-    });
-}
-
-// (dloss, logits, teacher_logits, teacher_index, labels | None, row statistics, temperature, alpha, ignore_index,
-// reduction) -> dlogits
-PyObject *distill_backward(PyObject *, PyObject *const *args, Py_ssize_t n)
-{
-    return guarded([&] {
-        Args g{Distill::kCall, args, n};
-        g.expect(10);
+        op.take(logits, top, index, labels, temperature, alpha, ignore, static_cast<int>(reduction));
+        Tensor grad;
+        const auto [loss, stats] = op.forward(true, grad);
+        ctx->save_for_backward({logits, top, index, labels, stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["alpha"] = alpha;
+        ctx->saved_data["ignore"] = ignore;
+        ctx->saved_data["reduction"] = reduction;
+        if (grad.defined()) {
+            ctx->saved_data["grad"] = grad;
+            ctx->saved_data["captured"] = op.captured;
+        }
+        return loss;
+    }
+    static tensor_list backward(AutogradContext *ctx, tensor_list grads)
+    {
+        first_order(Distill::kCall);
+        const auto saved = ctx->get_saved_variables();
         Distill op;
-        Tensor dloss = g.tensor();
-        const Tensor logits = g.tensor(), top = g.tensor(), index = g.tensor();
-        const Maybe labels = g.maybe();
-        Tensor stats = g.tensor();
-        const Maybe dloss_ = dloss, top_ = top, index_ = index, stats_ = stats;
-        const double temperature = g.real(), alpha = g.real();
-        const long long ignore = g.integer();
-        op.take(logits, top, index, labels, temperature, alpha, ignore, static_cast<int>(g.integer()));
-        const OnDevice on(Distill::kCall, logits, {&dloss_, &top_, &index_, &labels, &stats_});
-        op.lay_out();
-        dloss = dloss.to(at::kFloat).contiguous();
-        Tensor dlogits = at::empty(logits.sizes(), logits.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
-        op.d.dloss = dloss.data_ptr<float>();
-        op.d.dloss_row = op.d.reduction == 0 ? 1 : 0;
-        op.d.row_stats = stats.data_ptr<float>();
-        op.d.dlogits = dlogits.data_ptr();
-        int rc;
-        WITHOUT_GIL(rc, stdmlc_distill_backward(&op.d, on.index(), on.stream()));
-        done(rc);
-        return THPVariable_Wrap(dlogits);
-    });
-}
+        op.take(saved[0], saved[1], saved[2], saved[3], ctx->saved_data["temperature"].toDouble(),
+                ctx->saved_data["alpha"].toDouble(), ctx->saved_data["ignore"].toInt(),
+                static_cast<int>(ctx->saved_data["reduction"].toInt()));
+        const OnDevice on(Distill::kCall, op.logits, {&grads[0]});
+        const Tensor dloss = grads[0].to(at::kFloat).contiguous();
+        Tensor dlogits;
+        const auto held = ctx->saved_data.find("grad");
+        // The forward pass's gradient, for the first who asks.  It is multiplied in place, so a graph that is captured
+        // takes only one that its own replays write anew.
+        if (held != ctx->saved_data.end() &&
+            (stdmlc_stream_capturing(on.stream()) == 0) == !ctx->saved_data["captured"].toBool()) {
+            dlogits = held->second.toTensor();
+            ctx->saved_data.erase("grad");
+            done(stdmlc_distill_scale(dlogits.data_ptr(), dlogits.numel(), op.d.dt, dloss.data_ptr<float>(), on.index(), on.stream()));
+        } else {
+            dlogits = op.empty_grad();
+            op.lay_out();
+            op.d.dloss = dloss.data_ptr<float>();
+            op.d.dloss_row = op.d.reduction == 0 ? 1 : 0;
+            op.d.row_stats = saved[4].data_ptr<float>();
+            op.d.dlogits = dlogits.data_ptr();
+            done(stdmlc_distill_backward(&op.d, on.index(), on.stream()));
+        }
+        return {dlogits, {}, {}, {}, {}, {}, {}, {}};
+    }
+};
 
 // ------------------------------------------------------------ gated projection
 struct Gated {
     static constexpr const char *kCall = "gated_linear";
     stdmlc_gated a{};
-    Tensor x, w_gate, w_up;
-    Maybe b_gate, b_up;
+    Tensor x, w_gate, w_up, b_gate, b_up;
 
-    void take(const Tensor &x_, const Tensor &w_gate_, const Tensor &w_up_, const Maybe &b_gate_, const Maybe &b_up_,
+    void take(const Tensor &x_, const Tensor &w_gate_, const Tensor &w_up_, const Tensor &b_gate_, const Tensor &b_up_,
               int act)
     {
         x = x_;
@@ -529,113 +479,221 @@ struct Gated {
         if (a.hidden > (1ll << 20) || a.ffn > (1ll << 20) || a.tokens > (1ll << 22)) {
             refuse(kCall, "at most 2^22 tokens, 2^20 hidden and 2^20 ffn");
         }
-        if (b_gate.has_value() != b_up.has_value()) { refuse(kCall, "both biases or none"); }
-        for (const Maybe *b : {&b_gate, &b_up}) {
-            if (*b && ((*b)->dim() != 1 || (*b)->size(0) != a.ffn)) {
-                refuse(kCall, "biases of (" + std::to_string(a.ffn) + ",) expected, got " + shape_of(**b));
+        if (b_gate.defined() != b_up.defined()) { refuse(kCall, "both biases or none"); }
+        for (const Tensor *b : {&b_gate, &b_up}) {
+            if (b->defined() && (b->dim() != 1 || b->size(0) != a.ffn)) {
+                refuse(kCall, "biases of (" + std::to_string(a.ffn) + ",) expected, got " + shape_of(*b));
             }
         }
-        const Maybe wg = w_gate, wu = w_up;
-        for (const Maybe *t : std::initializer_list<const Maybe *>{&wg, &wu, &b_gate, &b_up}) {
-            if (*t && (*t)->scalar_type() != x.scalar_type()) {
-                refuse(kCall, "weights and biases must have the input's dtype", PyExc_TypeError);
+        for (const Tensor *t : {&w_gate, &w_up, &b_gate, &b_up}) {
+            if (t->defined() && t->scalar_type() != x.scalar_type()) {
+                refuse_type(kCall, "weights and biases must have the input's dtype");
             }
         }
         a.act = act;
     }
     void lay_out()
     {
-        const void *p;
-        x = matrix_of(x, &p, &a.x_row);
-        a.x = p;
-        w_gate = matrix_of(w_gate, &p, &a.w_gate_row);
-        a.w_gate = p;
-        w_up = matrix_of(w_up, &p, &a.w_up_row);
-        a.w_up = p;
-        for (Maybe *b : {&b_gate, &b_up}) {
-            if (*b) { *b = (*b)->contiguous(); }
+        x = matrix_of(x, &a.x, &a.x_row);
+        w_gate = matrix_of(w_gate, &a.w_gate, &a.w_gate_row);
+        w_up = matrix_of(w_up, &a.w_up, &a.w_up_row);
+        for (Tensor *b : {&b_gate, &b_up}) {
+            if (b->defined()) { *b = b->contiguous(); }
         }
         a.b_gate = ptr_of(b_gate);
         a.b_up = ptr_of(b_up);
     }
+    // h, and what a backward pass needs, if one follows
+    std::pair<Tensor, Tensor> forward(bool follows)
+    {
+        const OnDevice on(kCall, x, {&w_gate, &w_up, &b_gate, &b_up});
+        std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = a.ffn;
+        const Tensor like = x;
+        lay_out();
+        Tensor h = at::empty(shape, like.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous)), saved;
+        a.h = h.data_ptr();
+        if (follows) {
+            saved = bytes_like(like, stdmlc_gated_saved(&a));
+            a.saved = saved.data_ptr();
+        }
+        const Tensor work = bytes_like(like, stdmlc_gated_workspace(&a, 0));
+        a.workspace = work.data_ptr();
+        done(stdmlc_gated_forward(&a, on.index(), on.stream()));
+        return {h, saved};
+    }
 };
 
-// (x, w_gate, w_up, b_gate | None, b_up | None, activation, whether a backward pass follows) -> (h, saved | None)
-PyObject *gated_forward(PyObject *, PyObject *const *args, Py_ssize_t n)
+struct GatedFunction : torch::autograd::Function<GatedFunction> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w_gate, const Tensor &w_up, const Maybe &b_gate_,
+                          const Maybe &b_up_, int64_t act)
+    {
+        const Tensor b_gate = given(b_gate_), b_up = given(b_up_);
+        Gated op;
+        op.take(x, w_gate, w_up, b_gate, b_up, static_cast<int>(act));
+        const auto [h, saved] = op.forward(true);
+        ctx->save_for_backward({x, w_gate, w_up, b_gate, b_up, saved});
+        ctx->saved_data["act"] = act;
+        return h;
+    }
+    static tensor_list backward(AutogradContext *ctx, tensor_list grads)
+    {
+        first_order(Gated::kCall);
+        const auto saved = ctx->get_saved_variables();
+        Gated op;
+        op.take(saved[0], saved[1], saved[2], saved[3], saved[4], static_cast<int>(ctx->saved_data["act"].toInt()));
+        const OnDevice on(Gated::kCall, op.x, {&grads[0]});
+        op.lay_out();
+        const Tensor dh = matrix_of(grads[0], &op.a.dh, &op.a.dh_row);
+        op.a.saved = saved[5].data_ptr();
+        const auto packed = saved[0].options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+        tensor_list out(6);
+        for (size_t i = 0; i < 5; ++i) {
+            if (saved[i].defined() && ctx->needs_input_grad(i)) { out[i] = at::empty(saved[i].sizes(), packed); }
+        }
+        op.a.dx = ptr_of(out[0]);
+        op.a.dw_gate = ptr_of(out[1]);
+        op.a.dw_up = ptr_of(out[2]);
+        op.a.db_gate = ptr_of(out[3]);
+        op.a.db_up = ptr_of(out[4]);
+        const Tensor work = bytes_like(saved[0], stdmlc_gated_workspace(&op.a, 1));
+        op.a.workspace = work.data_ptr();
+        done(stdmlc_gated_backward(&op.a, on.index(), on.stream()));
+        return out;
+    }
+};
+
+// ------------------------------------------------------------ from Python
+struct Raised {
+};  // a Python exception is set
+
+struct Args {
+    const char *call;
+    PyObject *const *a;
+    Py_ssize_t n;
+    int i = 0;
+
+    void expect(Py_ssize_t want) const
+    {
+        if (n != want) { refuse_type(call, std::to_string(want) + " arguments expected"); }
+    }
+    Tensor optional()  // undefined for None
+    {
+        PyObject *o = a[i++];
+        if (o == Py_None) { return {}; }
+        if (!THPVariable_Check(o)) { refuse_type(call, std::string("tensor expected, got ") + Py_TYPE(o)->tp_name); }
+        return THPVariable_Unpack(o);
+    }
+    Tensor tensor()
+    {
+        const Tensor t = optional();
+        if (!t.defined()) { refuse_type(call, "tensor expected, got None"); }
+        return t;
+    }
+    long long integer()
+    {
+        const long long v = PyLong_AsLongLong(a[i++]);
+        if (v == -1 && PyErr_Occurred()) { throw Raised{}; }
+        return v;
+    }
+    double real()
+    {
+        const double v = PyFloat_AsDouble(a[i++]);
+        if (v == -1.0 && PyErr_Occurred()) { throw Raised{}; }
+        return v;
+    }
+};
+
+struct WithoutGil {
+    PyThreadState *state = PyEval_SaveThread();
+    ~WithoutGil() { PyEval_RestoreThread(state); }
+};
+
+template <typename F>
+PyObject *guarded(F f)
+{
+    try {
+        return THPVariable_Wrap(f());
+    } catch (const Raised &) {
+    } catch (const c10::ValueError &e) {
+        PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
+    } catch (const c10::TypeError &e) {
+        PyErr_SetString(PyExc_TypeError, e.what_without_backtrace());
+    } catch (const c10::OutOfMemoryError &e) {
+        PyObject *torch = PyImport_ImportModule("torch"), *kind = nullptr;
+        if (torch != nullptr) { kind = PyObject_GetAttrString(torch, "OutOfMemoryError"); }
+        if (kind != nullptr) { PyErr_SetString(kind, e.what_without_backtrace()); }
+        Py_XDECREF(kind);
+        Py_XDECREF(torch);
+    } catch (const c10::Error &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
+    } catch (const std::exception &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
+    }
+    return nullptr;
+}
+
+// (x, residual | None, weight | None, bias | None, groups, eps, activation) -> y
+PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
     return guarded([&] {
-        Args g{Gated::kCall, args, n};
+        Args g{Norm::kCall, args, n};
         g.expect(7);
-        Gated op;
-        const Tensor x = g.tensor(), wg = g.tensor(), wu = g.tensor();
-        const Maybe bg = g.maybe(), bu = g.maybe(), wg_ = wg, wu_ = wu;
-        op.take(x, wg, wu, bg, bu, static_cast<int>(g.integer()));
-        const OnDevice on(Gated::kCall, x, {&wg_, &wu_, &bg, &bu});
-        op.lay_out();
-        std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
-        shape.back() = op.a.ffn;
-        Tensor h = at::empty(shape, x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
-        op.a.h = h.data_ptr();
-        Maybe saved;
-        if (g.truth()) {
-            saved = bytes_like(x, stdmlc_gated_saved(&op.a));
-            op.a.saved = saved->data_ptr();
-        }
-        Tensor work = bytes_like(x, stdmlc_gated_workspace(&op.a, 0));
-        op.a.workspace = work.data_ptr();
-        int rc;
-        WITHOUT_GIL(rc, stdmlc_gated_forward(&op.a, on.index(), on.stream()));
-        done(rc);
-        return tuple_of({h, saved});
+        const Tensor x = g.tensor(), residual = g.optional(), weight = g.optional(), bias = g.optional();
+        const long long groups = g.integer();
+        const double eps = g.real();
+        const long long act = g.integer();
+        const WithoutGil free;
+        if (wanted({&x, &residual, &weight, &bias})) { return NormFunction::apply(x, maybe(residual), maybe(weight), maybe(bias), groups, eps, act); }
+        Norm op;
+        op.take(x, residual, weight, bias, groups, eps, static_cast<int>(act));
+        return op.forward().first;
     });
 }
 
-// (dh, x, w_gate, w_up, b_gate | None, b_up | None, saved, activation, want dx, want dw_gate, want dw_up, want
-// db_gate, want db_up) -> those
-PyObject *gated_backward(PyObject *, PyObject *const *args, Py_ssize_t n)
+// (logits, teacher_logits, teacher_index, labels | None, temperature, alpha, ignore_index, reduction) -> loss
+PyObject *distill_loss(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    return guarded([&] {
+        Args g{Distill::kCall, args, n};
+        g.expect(8);
+        const Tensor logits = g.tensor(), top = g.tensor(), index = g.tensor(), labels = g.optional();
+        const double temperature = g.real(), alpha = g.real();
+        const long long ignore = g.integer(), reduction = g.integer();
+        const WithoutGil free;
+        if (top.requires_grad()) { refuse(Distill::kCall, "teacher_logits are constants: a tensor without gradient expected"); }
+        if (wanted({&logits})) {
+            return DistillFunction::apply(logits, top, index, maybe(labels), temperature, alpha, ignore, reduction);
+        }
+        Distill op;
+        op.take(logits, top, index, labels, temperature, alpha, ignore, static_cast<int>(reduction));
+        Tensor none;
+        return op.forward(false, none).first;
+    });
+}
+
+// (x, w_gate, w_up, b_gate | None, b_up | None, activation) -> h
+PyObject *gated_linear(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
     return guarded([&] {
         Args g{Gated::kCall, args, n};
-        g.expect(13);
+        g.expect(6);
+        const Tensor x = g.tensor(), wg = g.tensor(), wu = g.tensor(), bg = g.optional(), bu = g.optional();
+        const long long act = g.integer();
+        const WithoutGil free;
+        if (wanted({&x, &wg, &wu, &bg, &bu})) { return GatedFunction::apply(x, wg, wu, maybe(bg), maybe(bu), act); }
         Gated op;
-        Tensor dh = g.tensor();
-        const Tensor x = g.tensor(), wg = g.tensor(), wu = g.tensor();
-        const Maybe bg = g.maybe(), bu = g.maybe();
-        Tensor saved = g.tensor();
-        const Maybe dh_ = dh, wg_ = wg, wu_ = wu, saved_ = saved;
-        op.take(x, wg, wu, bg, bu, static_cast<int>(g.integer()));
-        const OnDevice on(Gated::kCall, x, {&dh_, &wg_, &wu_, &bg, &bu, &saved_});
-        op.lay_out();
-        dh = matrix_of(dh, &op.a.dh, &op.a.dh_row);
-        op.a.saved = saved.data_ptr();
-        const auto packed = x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
-        Maybe dx, dwg, dwu, dbg, dbu;
-        if (g.truth()) { dx = at::empty(x.sizes(), packed); }
-        if (g.truth()) { dwg = at::empty(wg.sizes(), packed); }
-        if (g.truth()) { dwu = at::empty(wg.sizes(), packed); }
-        if (g.truth()) { dbg = at::empty({op.a.ffn}, packed); }
-        if (g.truth()) { dbu = at::empty({op.a.ffn}, packed); }
-        op.a.dx = ptr_of(dx);
-        op.a.dw_gate = ptr_of(dwg);
-        op.a.dw_up = ptr_of(dwu);
-        op.a.db_gate = ptr_of(dbg);
-        op.a.db_up = ptr_of(dbu);
-        Tensor work = bytes_like(x, stdmlc_gated_workspace(&op.a, 1));
-        op.a.workspace = work.data_ptr();
-        int rc;
-        WITHOUT_GIL(rc, stdmlc_gated_backward(&op.a, on.index(), on.stream()));
-        done(rc);
-        return tuple_of({dx, dwg, dwu, dbg, dbu});
+        op.take(x, wg, wu, bg, bu, static_cast<int>(act));
+        return op.forward(false).first;
     });
 }
 
 PyMethodDef kMethods[] = {
-    {"norm_forward", reinterpret_cast<PyCFunction>(norm_forward), METH_FASTCALL, nullptr},
-    {"norm_backward", reinterpret_cast<PyCFunction>(norm_backward), METH_FASTCALL, nullptr},
-    {"distill_forward", reinterpret_cast<PyCFunction>(distill_forward), METH_FASTCALL, nullptr},
-    {"distill_backward", reinterpret_cast<PyCFunction>(distill_backward), METH_FASTCALL, nullptr},
-    {"gated_forward", reinterpret_cast<PyCFunction>(gated_forward), METH_FASTCALL, nullptr},
-    {"gated_backward", reinterpret_cast<PyCFunction>(gated_backward), METH_FASTCALL, nullptr},
+    {"group_norm", reinterpret_cast<PyCFunction>(group_norm), METH_FASTCALL, nullptr},
+    {"distill_loss", reinterpret_cast<PyCFunction>(distill_loss), METH_FASTCALL, nullptr},
+    {"gated_linear", reinterpret_cast<PyCFunction>(gated_linear), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 }  // namespace

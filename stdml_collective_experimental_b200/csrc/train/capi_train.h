@@ -60,17 +60,21 @@ typedef struct {
     float temperature, alpha;
     int reduction;     /* 0: each row, 1: sum, 2: mean over the rows that count */
     float *loss;       /* one value, or one of each row */
-    float *row_stats;  /* [rows][4]: log-sum-exp of z, of z / t, of the teacher's top, weight of the row */
+    float *row_stats;  /* [rows][5]: maximum, the two sums, the teacher's log-sum, weight of the row */
     void *workspace;   /* stdmlc_distill_workspace() bytes */
     /* backward */
     const float *dloss; /* one value, or one of each row (dloss_row apart) */
     long long dloss_row;
-    void *dlogits;      /* rows x classes, packed */
+    /* rows x classes, packed.  In a forward call (bf16 and f32, reductions to one value): null, or where to write the
+     * gradient of the loss, which stdmlc_distill_scale() multiplies by the loss's own gradient later. */
+    void *dlogits;
 } stdmlc_distill;
 
 long long stdmlc_distill_workspace(const stdmlc_distill *a);
 int stdmlc_distill_forward(const stdmlc_distill *a, int device, void *stream);
 int stdmlc_distill_backward(const stdmlc_distill *a, int device, void *stream);
+int stdmlc_distill_scale(void *grad, long long count, int dt, const float *by, int device, void *stream);
+int stdmlc_stream_capturing(void *stream); /* 1: a graph is being captured on it */
 
 /* h = act(g) * u, g = x w_gate^T + b_gate, u = x w_up^T + b_up. */
 typedef struct {

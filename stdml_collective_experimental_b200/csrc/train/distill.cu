@@ -1,18 +1,35 @@
 // The distillation loss against a teacher's top logits, forward and backward.
 //
 // A row with logits z, teacher's logits v_j at classes k_j, temperature t, label y:
-//   p_j = softmax(v / t)_j;  l = log sum exp z;  m = log sum exp(z / t)
-//   loss = a * (l - z_y) + b * t^2 * sum_j p_j * (log p_j - z_kj / t + m)
-//   dz_i = a * (exp(z_i - l) - [i = y]) + b * t * (exp(z_i / t - m) * [any p] - sum_{kj = i} p_j)
+//   p_j = softmax(v / t)_j;  M = max z;  s = sum exp(z - M);  S = sum exp((z - M) / t)
+//   loss = a * (log s - (z_y - M)) + b * t^2 * sum_j p_j * (log p_j - (z_kj - M) / t + log S)
+//   dz_i = a * (exp(z_i - M) / s - [i = y]) + b * t * (exp((z_i - M) / t) / S * [any p] - sum_{kj = i} p_j)
 // with b = 1 - a, or a = 0 and b = 1 without labels.
+//
+// Bytes bound it: the logits once in, the gradient once out.  A block (for few rows a cluster of blocks) takes a row,
+// walks it once with running maximum and sums, and, where the caller wants gradients, a second time to write
+// them: the row comes from the L2 then, since the rows in work at a time are fewer than fit there.  The classes that
+// the teacher or the label names are corrected afterwards.
 #include "dispatch.cuh"
 #include "host.hpp"
+#include "ptx.cuh"
 
 namespace stdml::collective::train
 {
 namespace
 {
-constexpr int kThreads = 256;
+constexpr int kUnroll = 4;       // vectors of 16 bytes that a thread has on their way
+constexpr int kCountBlocks = 256;
+constexpr int kMostCluster = 8;
+
+struct Args {
+    stdmlc_distill d;
+    float *row_loss;
+    int *counts;           // rows that count, of each block of the counting kernel; then the ticket
+    int count_blocks;      // 0: every row weighs one
+    void *grad;            // null: none wanted in the forward pass
+    int cluster;
+};
 
 __device__ __forceinline__ long long index_at(const stdmlc_distill &d, long long r, int j)
 {
@@ -29,128 +46,397 @@ __device__ __forceinline__ long long label_at(const stdmlc_distill &d, long long
 // Whether the teacher has an entry in row r (a warp asks).
 __device__ __forceinline__ bool has_entry(const stdmlc_distill &d, long long r)
 {
-    bool any = false;
-    for (int j = threadIdx.x & 31; j < d.top_count; j += 32) {
-        const long long k = index_at(d, r, j);
-        any = any || (k >= 0 && k < d.classes && load_any(d.top, r * d.top_row + j, d.top_dt) != -INFINITY);
+    for (int base = 0; base < d.top_count; base += 32) {
+        const int j = base + (threadIdx.x & 31);
+        bool in = false;
+        if (j < d.top_count) {
+            const long long k = index_at(d, r, j);
+            in = k >= 0 && k < d.classes && load_any(d.top, r * d.top_row + j, d.top_dt) * (1.f / d.temperature) != -INFINITY;
+        }
+        if (__any_sync(0xffffffffu, in)) { return true; }
     }
-    return __any_sync(0xffffffffu, any);
+    return false;
 }
 
-// The weight of every row: 1 or 1 / (rows that count), 0 where it does not count.
-__global__ void weights_kernel(stdmlc_distill d)
+// How many rows count: one number for each block, which the rows' blocks add up.
+__global__ void __launch_bounds__(1024) count_kernel(stdmlc_distill d, int *counts)
 {
-    __shared__ long long slots[32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    long long live = 0;
-    for (long long r = warp; r < d.rows; r += warps) {
-        const bool counts = d.labels != nullptr ? label_at(d, r) >= 0 : has_entry(d, r);
-        if (lane == 0) { d.row_stats[4 * r + 3] = counts ? 1.f : 0.f; }
-        live += counts && lane == 0 ? 1 : 0;
+    __shared__ int slots[32];
+    int live = 0;
+    if (d.labels != nullptr) {
+        for (long long r = blockIdx.x * 1024ll + threadIdx.x; r < d.rows; r += gridDim.x * 1024ll) {
+            live += label_at(d, r) >= 0 ? 1 : 0;
+        }
+    } else {
+        const int lane = threadIdx.x & 31;
+        for (long long r = blockIdx.x * 32ll + (threadIdx.x >> 5); r < d.rows; r += gridDim.x * 32ll) {
+            const bool counts_ = has_entry(d, r);
+            live += counts_ && lane == 0 ? 1 : 0;
+        }
     }
     live = block_sum(live, slots);
-    if (d.reduction != 2) { return; }
-    const float each = 1.f / static_cast<float>(live > 0 ? live : 1);
-    for (long long r = threadIdx.x; r < d.rows; r += blockDim.x) { d.row_stats[4 * r + 3] *= each; }
+    if (threadIdx.x == 0) {
+        counts[blockIdx.x] = live;
+        if (blockIdx.x == 0) { counts[kCountBlocks] = 0; }  // the ticket
+    }
 }
 
+// A row, or a block's share of it: single elements up to a 16-byte boundary, vectors, single elements.
 template <typename T>
-__global__ void rows_kernel(stdmlc_distill d, float *row_loss)
-{
-    __shared__ float slots[32];
-    const long long r = blockIdx.x;
-    const T *z = static_cast<const T *>(d.logits) + r * d.logits_row;
-    const float inv_t = 1.f / d.temperature;
-    float *st = d.row_stats + 4 * r;
-    float most = -INFINITY;
-    for (long long i = threadIdx.x; i < d.classes; i += blockDim.x) { most = fmaxf(most, to_f32(z[i])); }
-    most = block_max(most, slots);
-    float s1 = 0, st_ = 0;
-    for (long long i = threadIdx.x; i < d.classes; i += blockDim.x) {
-        const float v = to_f32(z[i]);
-        s1 += expf(v - most);
-        st_ += expf((v - most) * inv_t);
+struct Share {
+    static constexpr int kPer = 16 / sizeof(T);
+    const T *z;
+    long long head, vectors, from, to, tail;  // vectors [from, to) are the block's; elements from `tail` on the last block's
+
+    __device__ __forceinline__ Share(const T *row, long long classes, int part, int parts) : z(row)
+    {
+        head = min(classes, static_cast<long long>((16u - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / static_cast<int>(sizeof(T)));
+        vectors = (classes - head) / kPer;
+        from = vectors * part / parts;
+        to = vectors * (part + 1) / parts;
+        tail = head + vectors * kPer;
     }
-    const float lse = most + logf(block_sum(s1, slots)), lset = most * inv_t + logf(block_sum(st_, slots));
+    // f(element index, values, how many), for all of the block's; `several`: kUnroll vectors at once
+    template <typename F>
+    __device__ __forceinline__ void each(long long classes, bool first, bool last, F f) const
+    {
+        if (first && threadIdx.x < head) { f.one(threadIdx.x, to_f32(z[threadIdx.x])); }
+        const uint4 *v = reinterpret_cast<const uint4 *>(z + head);
+        long long i = from + threadIdx.x;
+        for (; i + (kUnroll - 1) * blockDim.x < to; i += kUnroll * blockDim.x) {
+            uint4 raw[kUnroll];
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) { raw[k] = v[i + k * blockDim.x]; }
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) { f.vector(head + (i + k * blockDim.x) * kPer, raw[k]); }
+        }
+        for (; i < to; i += blockDim.x) { f.vector(head + i * kPer, v[i]); }
+        if (last && tail + threadIdx.x < classes) { f.one(tail + threadIdx.x, to_f32(z[tail + threadIdx.x])); }
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4 &raw, float (&v)[16 / sizeof(T)])
+{
+    const T *t = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) { v[i] = to_f32(t[i]); }
+}
+
+constexpr float kLowest = -3.402823466e38f;
+
+// Maximum and sums of what a thread has seen.
+struct Running {
+    float most = kLowest, hard = 0, soft = 0;
+
+    __device__ __forceinline__ void raise(float to, float c)
+    {
+        if (to > most) {
+            hard *= fast_exp2((most - to) * kLog2E);
+            soft *= fast_exp2((most - to) * c);
+            most = to;
+        }
+    }
+};
+
+template <typename T, bool kHard, bool kSoft>
+struct Walk {
+    Running &r;
+    float c;  // log2(e) / t
+
+    __device__ __forceinline__ void one(long long, float v)
+    {
+        r.raise(v, c);
+        add(v);
+    }
+    __device__ __forceinline__ void vector(long long, const uint4 &raw)
+    {
+        float v[16 / sizeof(T)];
+        unpack<T>(raw, v);
+        float most = v[0];
+#pragma unroll
+        for (int i = 1; i < static_cast<int>(16 / sizeof(T)); ++i) { most = fmaxf(most, v[i]); }
+        r.raise(most, c);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) { add(v[i]); }
+    }
+    __device__ __forceinline__ void add(float v)
+    {
+        // (the difference first: a product of its own could overflow at a mask's lowest value)
+        const float below = v - r.most;
+        if constexpr (kHard) { r.hard += fast_exp2(below * kLog2E); }
+        if constexpr (kSoft) { r.soft += fast_exp2(below * c); }
+    }
+};
+
+template <typename T, bool kHard, bool kSoft>
+struct Write {
+    T *dz;
+    float most, hard, soft, c;  // factors of the two exponentials
+    bool same;                  // the gradient's rows lie on the same boundaries as the logits'
+
+    __device__ __forceinline__ float grad(float v) const
+    {
+        const float below = v - most;
+        float g = 0;
+        if constexpr (kHard) { g += hard * fast_exp2(below * kLog2E); }
+        if constexpr (kSoft) { g += soft * fast_exp2(below * c); }
+        return g;
+    }
+    __device__ __forceinline__ void one(long long i, float v) { dz[i] = from_f32<T>(grad(v)); }
+    __device__ __forceinline__ void vector(long long i, const uint4 &raw)
+    {
+        float v[16 / sizeof(T)];
+        unpack<T>(raw, v);
+        __align__(16) T out[16 / sizeof(T)];
+#pragma unroll
+        for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k) { out[k] = from_f32<T>(grad(v[k])); }
+        if (same) {
+            __stcs(reinterpret_cast<uint4 *>(dz + i), *reinterpret_cast<const uint4 *>(out));
+        } else {
+#pragma unroll
+            for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k) { dz[i + k] = out[k]; }
+        }
+    }
+};
+
+// The teacher's probabilities of a row and their classes (-1: no entry), in shared memory; the logarithm of the sum of
+// exp(v / t), -inf without an entry.
+__device__ __forceinline__ float teacher_row(const stdmlc_distill &d, long long r, float *prob, int *cls, float *slots)
+{
+    const float inv_t = 1.f / d.temperature;
     float top = -INFINITY;
     for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
         const long long k = index_at(d, r, j);
-        if (k >= 0 && k < d.classes) { top = fmaxf(top, load_any(d.top, r * d.top_row + j, d.top_dt) * inv_t); }
+        const bool in = k >= 0 && k < d.classes;
+        const float v = in ? load_any(d.top, r * d.top_row + j, d.top_dt) * inv_t : -INFINITY;
+        cls[j] = in ? static_cast<int>(k) : -1;
+        prob[j] = v;
+        top = v > top || v != v ? v : top;  // (NaN stays)
     }
-    top = block_max(top, slots);
-    const bool some = top != -INFINITY;
-    float sp = 0;
-    for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
-        const long long k = index_at(d, r, j);
-        if (some && k >= 0 && k < d.classes) { sp += expf(load_any(d.top, r * d.top_row + j, d.top_dt) * inv_t - top); }
+    if (d.top_count <= 32) {
+        // one warp has them all
+        __syncthreads();
+        float lp = -INFINITY;
+        if (threadIdx.x < 32) {
+            const bool nan = __any_sync(0xffffffffu, top != top);
+            const float m = warp_max(top);
+            const float sum = warp_sum(threadIdx.x < d.top_count && m != -INFINITY ? expf(prob[threadIdx.x] - m) : 0.f);
+            lp = nan ? NAN : m == -INFINITY ? -INFINITY : m + logf(sum);
+            if (threadIdx.x == 0) { slots[32] = lp; }
+        }
+        __syncthreads();
+        return slots[32];
     }
-    const float lp = some ? top + logf(block_sum(sp, slots)) : -INFINITY;
-    float kl = 0;
-    for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
-        const long long k = index_at(d, r, j);
-        if (!some || k < 0 || k >= d.classes) { continue; }
-        const float logp = load_any(d.top, r * d.top_row + j, d.top_dt) * inv_t - lp;
-        if (logp != -INFINITY) { kl += expf(logp) * (logp - (to_f32(z[k]) * inv_t - lset)); }
-    }
-    kl = block_sum(kl, slots);
-    if (threadIdx.x != 0) { return; }
-    const float weight = st[3];
-    float loss = d.temperature * d.temperature * kl;
-    if (d.labels != nullptr) {
-        const long long y = label_at(d, r);
-        loss = (1.f - d.alpha) * loss + (y >= 0 ? d.alpha * (lse - to_f32(z[y])) : 0.f);
-    }
-    st[0] = lse;
-    st[1] = lset;
-    st[2] = lp;
-    row_loss[r] = weight != 0.f ? weight * loss : 0.f;
+    const bool nan = __syncthreads_or(top != top ? 1 : 0) != 0;
+    const float m = block_max(top, slots);
+    float sum = 0;
+    for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) { sum += m != -INFINITY ? expf(prob[j] - m) : 0.f; }
+    sum = block_sum(sum, slots);
+    return nan ? NAN : m == -INFINITY ? -INFINITY : m + logf(sum);
 }
 
-__global__ void total_kernel(const float *row_loss, long long rows, float *loss)
+// Gradients at the classes that teacher or label name, over what the walk has written.  `up`: the row's factor.
+template <typename T, bool kHard, bool kSoft>
+__device__ __forceinline__ void correct(const stdmlc_distill &d, const Write<T, kHard, kSoft> &w, const T *z, long long y, float hard, float soft,
+                                        const float *prob, const int *cls, int lead, int step)
 {
-    __shared__ double slots[32];
-    double sum = 0;
-    for (long long r = threadIdx.x; r < rows; r += blockDim.x) { sum += row_loss[r]; }
-    sum = block_sum(sum, slots);
-    if (threadIdx.x == 0) { *loss = static_cast<float>(sum); }
+    bool y_named = false;
+    for (int j = lead; j < d.top_count; j += step) {
+        const int k = cls[j];
+        if (k < 0) { continue; }
+        bool again = false;  // a class that is named twice is written once, for both
+        for (int i = 0; i < j; ++i) { again = again || cls[i] == k; }
+        if (again) { continue; }
+        float p = prob[j];
+        for (int i = j + 1; i < d.top_count; ++i) { p += cls[i] == k ? prob[i] : 0.f; }
+        w.dz[k] = from_f32<T>(w.grad(to_f32(z[k])) - soft * p - (k == y ? hard : 0.f));
+    }
+    if (y >= 0 && lead == 0) {
+        for (int j = 0; j < d.top_count; ++j) { y_named = y_named || cls[j] == y; }
+        if (!y_named) { w.dz[y] = from_f32<T>(w.grad(to_f32(z[y])) - hard); }
+    }
+}
+
+constexpr int kStats = 5;  // of a row: maximum, the two sums, the teacher's log-sum, the row's weight
+
+// A row's gradient from its statistics.  kBlocks: threads of the cluster share it.
+template <typename T, bool kHard, bool kSoft>
+__device__ __forceinline__ void write_row(const stdmlc_distill &d, long long r, void *grad, float up, float most, float hard_sum,
+                                          float soft_sum, float lp, const float *prob, const int *cls, int part, int parts)
+{
+    const T *z = static_cast<const T *>(d.logits) + r * d.logits_row;
+    T *dz = static_cast<T *>(grad) + r * d.classes;
+    const bool labels = d.labels != nullptr, some = lp != -INFINITY;
+    const float hard = labels ? up * d.alpha : 0.f, soft = some ? (labels ? up * (1.f - d.alpha) : up) * d.temperature : 0.f;
+    const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0;
+    const Write<T, kHard, kSoft> w{dz, most, hard / hard_sum, soft != 0.f ? soft / soft_sum : 0.f, kLog2E / d.temperature, same};
+    Share<T>(z, d.classes, part, parts).each(d.classes, part == 0, part == parts - 1, w);
+    if (parts > 1) {
+        cluster_sync();
+    } else {
+        __syncthreads();
+    }
+    const long long y = labels ? label_at(d, r) : -1;
+    if (part == 0) { correct<T, kHard, kSoft>(d, w, z, y, kHard ? hard : 0.f, kSoft ? soft : 0.f, prob, cls, threadIdx.x, blockDim.x); }
 }
 
 template <typename T>
-__global__ void grad_kernel(stdmlc_distill d)
+__device__ __forceinline__ void zero_row(T *dz, long long classes, int part, int parts)
+{
+    const long long from = classes * part / parts, to = classes * (part + 1) / parts;
+    for (long long i = from + threadIdx.x; i < to; i += blockDim.x) { dz[i] = from_f32<T>(0.f); }
+}
+
+// kHard, kSoft: whether either softmax of the student is needed.
+template <typename T, bool kHard, bool kSoft>
+__global__ void __launch_bounds__(1024) rows_kernel(Args a)
 {
     extern __shared__ float held[];  // the teacher's probabilities, then their classes
-    const long long r = blockIdx.x;
+    __shared__ float slots[33];
+    __shared__ float shares[3 * kMostCluster];
+    __shared__ int counted;
+    const stdmlc_distill &d = a.d;
+    const int parts = a.cluster, part = parts > 1 ? static_cast<int>(cta_rank()) : 0;
+    const long long r = blockIdx.x / parts;
     const T *z = static_cast<const T *>(d.logits) + r * d.logits_row;
-    T *dz = static_cast<T *>(d.dlogits) + r * d.classes;
-    const float *st = d.row_stats + 4 * r;
-    const float inv_t = 1.f / d.temperature, weight = st[3];
+    float *prob = held;
+    int *cls = reinterpret_cast<int *>(held + d.top_count);
+    int live = 0;
+    if (threadIdx.x < a.count_blocks) { live = a.counts[threadIdx.x]; }
+    for (int i = threadIdx.x + blockDim.x; i < a.count_blocks; i += blockDim.x) { live += a.counts[i]; }
+    const float lp = teacher_row(d, r, prob, cls, slots);
+    const long long y = d.labels != nullptr ? label_at(d, r) : -1;
+    const bool counts = d.labels != nullptr ? y >= 0 : lp != -INFINITY;
+    if (!counts) {  // (the same in all blocks of the row)
+        if (a.grad != nullptr) { zero_row(static_cast<T *>(a.grad) + r * d.classes, d.classes, part, parts); }
+        if (part == 0 && threadIdx.x == 0) {
+            d.row_stats[kStats * r + 4] = 0.f;
+            a.row_loss[r] = 0.f;
+        }
+    } else {
+        float weight = 1.f;
+        if (a.count_blocks > 0) {
+            live = block_sum(live, reinterpret_cast<int *>(slots));
+            weight = 1.f / static_cast<float>(live);
+        }
+        const float c = kLog2E / d.temperature;
+        Running run;
+        Share<T>(z, d.classes, part, parts).each(d.classes, part == 0, part == parts - 1, Walk<T, kHard, kSoft>{run, c});
+        float most = block_max(run.most, slots);
+        const bool bad = __syncthreads_or(run.hard != run.hard || run.soft != run.soft ? 1 : 0) != 0;  // (fmaxf drops NaN)
+        run.raise(most, c);
+        float hard = kHard ? block_sum(run.hard, slots) : 1.f, soft = kSoft ? block_sum(run.soft, slots) : 1.f;
+        if (bad) { hard = soft = NAN; }
+        if (parts > 1) {
+            // every block gets every block's
+            if (threadIdx.x < parts) {
+                const uint32_t at = smem_at(shares + 3 * part);
+                uint32_t there;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(static_cast<uint32_t>(threadIdx.x)));
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(most) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there + 4), "f"(hard) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there + 8), "f"(soft) : "memory");
+            }
+            cluster_sync();
+            float all = kLowest;
+            for (int k = 0; k < parts; ++k) { all = fmaxf(all, shares[3 * k]); }
+            hard = soft = 0;
+            for (int k = 0; k < parts; ++k) {
+                hard += shares[3 * k + 1] * (kHard ? fast_exp2((shares[3 * k] - all) * kLog2E) : 1.f / parts);
+                soft += shares[3 * k + 2] * (kSoft ? fast_exp2((shares[3 * k] - all) * c) : 1.f / parts);
+            }
+            most = all;
+        }
+        // the teacher's side
+        const float inv_t = 1.f / d.temperature, log_soft = kSoft ? logf(soft) : 0.f;
+        float kl = 0;
+        for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
+            const float logp = prob[j] - lp, p = cls[j] >= 0 ? expf(logp) : 0.f;
+            if (kSoft && lp != -INFINITY && cls[j] >= 0 && logp != -INFINITY) {
+                kl += p * (logp - ((to_f32(z[cls[j]]) - most) * inv_t - log_soft));
+            }
+            prob[j] = lp != -INFINITY ? p : 0.f;
+        }
+        if (part == 0) {
+            kl = block_sum(kl, slots);
+            if (threadIdx.x == 0) {
+                float loss = d.temperature * d.temperature * kl;
+                if (d.labels != nullptr) {
+                    loss = (kSoft ? (1.f - d.alpha) * loss : 0.f) + (kHard ? d.alpha * (logf(hard) - (to_f32(z[y]) - most)) : 0.f);
+                }
+                float *st = d.row_stats + kStats * r;
+                st[0] = most;
+                st[1] = hard;
+                st[2] = soft;
+                st[3] = lp;
+                st[4] = weight;
+                a.row_loss[r] = weight * loss;
+            }
+        }
+        __syncthreads();
+        if (a.grad != nullptr) { write_row<T, kHard, kSoft>(d, r, a.grad, weight, most, hard, soft, lp, prob, cls, part, parts); }
+    }
+    // Whoever comes last adds up the rows, in their order.
+    if (d.reduction == 0 || part != 0) { return; }
+    if (threadIdx.x == 0) {
+        __threadfence();
+        counted = atomicAdd(a.counts + kCountBlocks, 1);
+    }
+    __syncthreads();
+    if (counted != static_cast<int>(d.rows) - 1) { return; }
+    __threadfence();
+    __shared__ double sums[32];
+    double sum = 0;
+    for (long long i = threadIdx.x; i < d.rows; i += blockDim.x) { sum += __ldcg(a.row_loss + i); }
+    sum = block_sum(sum, sums);
+    if (threadIdx.x == 0) { *d.loss = static_cast<float>(sum); }
+}
+
+template <typename T, bool kHard, bool kSoft>
+__global__ void __launch_bounds__(1024) grad_kernel(Args a)
+{
+    extern __shared__ float held[];
+    __shared__ float slots[33];
+    const stdmlc_distill &d = a.d;
+    const int parts = a.cluster, part = parts > 1 ? static_cast<int>(cta_rank()) : 0;
+    const long long r = blockIdx.x / parts;
+    const float *st = d.row_stats + kStats * r;
+    const float weight = st[4];
     if (weight == 0.f) {
-        for (long long i = threadIdx.x; i < d.classes; i += blockDim.x) { dz[i] = from_f32<T>(0.f); }
+        zero_row(static_cast<T *>(a.grad) + r * d.classes, d.classes, part, parts);
         return;
     }
     const float up = weight * d.dloss[d.reduction == 0 ? r * d.dloss_row : 0];
-    const float lse = st[0], lset = st[1], lp = st[2];
-    const float hard = d.labels != nullptr ? up * d.alpha : 0.f;
-    const float soft = (d.labels != nullptr ? up * (1.f - d.alpha) : up) * d.temperature;
-    const bool some = lp != -INFINITY;
-    const long long y = d.labels != nullptr ? label_at(d, r) : -1;
     float *prob = held;
     int *cls = reinterpret_cast<int *>(held + d.top_count);
-    for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
-        const long long k = index_at(d, r, j);
-        const bool in = some && k >= 0 && k < d.classes;
-        cls[j] = in ? static_cast<int>(k) : -1;
-        prob[j] = in ? expf(load_any(d.top, r * d.top_row + j, d.top_dt) * inv_t - lp) : 0.f;
+    const float lp = part == 0 ? teacher_row(d, r, prob, cls, slots) : st[3];
+    if (part == 0) {
+        for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
+            prob[j] = cls[j] >= 0 && lp != -INFINITY ? expf(prob[j] - lp) : 0.f;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    for (long long i = threadIdx.x; i < d.classes; i += blockDim.x) {
-        const float v = to_f32(z[i]);
-        float p = 0;
-        for (int j = 0; j < d.top_count; ++j) { p += cls[j] == static_cast<int>(i) ? prob[j] : 0.f; }
-        float g = some ? soft * (expf(v * inv_t - lset) - p) : 0.f;
-        if (hard != 0.f) { g += hard * (expf(v - lse) - (i == y ? 1.f : 0.f)); }
-        dz[i] = from_f32<T>(g);
+    write_row<T, kHard, kSoft>(d, r, a.grad, up, st[0], st[1], st[2], lp, prob, cls, part, parts);
+}
+
+// A gradient that the forward pass has written, times what came from above: nothing to do for one.
+template <typename T>
+__global__ void __launch_bounds__(512) scale_kernel(T *grad, long long many, const float *dloss)
+{
+    const float up = *dloss;
+    if (up == 1.f) { return; }
+    const long long first = blockIdx.x * 512ll + threadIdx.x, step = gridDim.x * 512ll;
+    constexpr int kPer = 16 / sizeof(T);
+    uint4 *v = reinterpret_cast<uint4 *>(grad);
+    for (long long i = first; i < many / kPer; i += step) {
+        uint4 raw = v[i];
+        T *t = reinterpret_cast<T *>(&raw);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) { t[k] = from_f32<T>(to_f32(t[k]) * up); }
+        v[i] = raw;
     }
+    for (long long i = many / kPer * kPer + first; i < many; i += step) { grad[i] = from_f32<T>(to_f32(grad[i]) * up); }
 }
 
 void check(const stdmlc_distill *d)
@@ -158,8 +444,8 @@ void check(const stdmlc_distill *d)
     require(d != nullptr, "distill_loss: null arguments");
     require(float_type(d->dt) && float_type(d->top_dt), "distill_loss: bf16, f16 or f32 expected");
     require(d->index_bytes == 4 || d->index_bytes == 8, "distill_loss: 32 or 64-bit indices expected");
-    require(d->rows >= 0 && d->rows < (1ll << 31) && d->classes > 0 && d->classes < (1ll << 31),
-            "distill_loss: bad sizes");
+    require(d->rows >= 0 && d->rows < (1ll << 28) && d->classes > 0 && d->classes < (1ll << 31),
+            "distill_loss: at most 2^28 rows of 2^31 classes");
     require(d->top_count >= 0 && d->top_count <= 4096, "distill_loss: at most 4096 teacher entries in a row");
     require(d->temperature > 0.f, "distill_loss: the temperature must be positive");
     require(d->reduction >= 0 && d->reduction <= 2, "distill_loss: unknown reduction");
@@ -167,6 +453,50 @@ void check(const stdmlc_distill *d)
     require(d->rows == 0 || d->top_count == 0 || (d->top != nullptr && d->index != nullptr),
             "distill_loss: null operand");
 }
+
+// How many blocks share a row, and their threads.
+//   Rows that are fewer than the SMs are spread over clusters, down to 4 KB for each block.
+//   A thread has about kUnroll vectors, in up to 1024 threads: with two such blocks on an SM, rows of 256 KB in
+//   work take 76 MB of the L2's 126.
+void launch_shape(const stdmlc_distill &d, int &cluster, int &threads)
+{
+    const long long vectors = (d.classes * element_size(d.dt) + 15) / 16;
+    cluster = 1;
+    while (cluster < kMostCluster && d.rows * cluster * 2 <= 2 * sm_count() && vectors / (cluster * 2) >= 256) { cluster *= 2; }
+    threads = 128;
+    while (threads < 1024 && threads * kUnroll * cluster < vectors) { threads *= 2; }
+}
+
+template <typename F>
+void by_need(const stdmlc_distill &d, F f)
+{
+    const bool hard = d.labels != nullptr && d.alpha != 0.f, soft = d.labels == nullptr || d.alpha != 1.f;
+    if (hard && soft) {
+        f(Int<1>{}, Int<1>{});
+    } else if (hard) {
+        f(Int<1>{}, Int<0>{});
+    } else {
+        f(Int<0>{}, Int<1>{});
+    }
+}
+
+template <typename Kernel>
+void launch_rows(Kernel kernel, const Args &a, int threads, cudaStream_t s)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned int>(a.d.rows * a.cluster));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = 8 * static_cast<size_t>(a.d.top_count);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {static_cast<unsigned int>(a.cluster), 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cuda_ok(cudaLaunchKernelEx(&cfg, kernel, a), "distill_loss: launch");
+}
+
+constexpr long long up16(long long n) { return (n + 15) / 16 * 16; }
 }  // namespace
 }  // namespace stdml::collective::train
 
@@ -175,7 +505,7 @@ using namespace stdml::collective::train;
 extern "C" long long stdmlc_distill_workspace(const stdmlc_distill *d)
 {
     if (d == nullptr || d->rows < 0) { return -1; }
-    return d->reduction == 0 ? 0 : 4 * d->rows;
+    return d->reduction == 0 ? 0 : up16(4 * d->rows) + 4 * (kCountBlocks + 1);
 }
 
 extern "C" int stdmlc_distill_forward(const stdmlc_distill *d, int device, void *stream)
@@ -184,15 +514,28 @@ extern "C" int stdmlc_distill_forward(const stdmlc_distill *d, int device, void 
         check(d);
         require(d->loss != nullptr || (d->rows == 0 && d->reduction == 0), "distill_loss: null operand");
         require(d->rows == 0 || d->reduction == 0 || d->workspace != nullptr, "distill_loss: null workspace");
+        require(d->dlogits == nullptr || (d->reduction != 0 && d->dt != kF16), "distill_loss: no gradient in the forward pass here");
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        float *row_loss = d->reduction == 0 ? d->loss : static_cast<float *>(d->workspace);
-        if (d->rows > 0) {
-            weights_kernel<<<1, 1024, 0, s>>>(*d);
-            by_dtype(d->dt, [&](auto t) {
-                rows_kernel<decltype(t)><<<static_cast<unsigned int>(d->rows), kThreads, 0, s>>>(*d, row_loss);
-            });
+        if (d->rows == 0) {
+            if (d->reduction != 0) { cuda_ok(cudaMemsetAsync(d->loss, 0, 4, s), "cudaMemsetAsync"); }
+            return;
         }
-        if (d->reduction != 0) { total_kernel<<<1, 1024, 0, s>>>(row_loss, d->rows, d->loss); }
+        Args a{*d, d->loss, nullptr, 0, d->dlogits, 1};
+        int threads;
+        launch_shape(*d, a.cluster, threads);
+        if (d->reduction != 0) {
+            a.row_loss = static_cast<float *>(d->workspace);
+            a.counts = reinterpret_cast<int *>(static_cast<char *>(d->workspace) + up16(4 * d->rows));
+            const long long each = d->labels != nullptr ? 1024 : 32, blocks = (d->rows + each - 1) / each;
+            const int used = static_cast<int>(blocks < kCountBlocks ? blocks : kCountBlocks);
+            count_kernel<<<static_cast<unsigned int>(used), 1024, 0, s>>>(*d, a.counts);
+            a.count_blocks = d->reduction == 2 ? used : 0;
+        }
+        by_dtype(d->dt, [&](auto t) {
+            by_need(*d, [&](auto hard, auto soft) {
+                launch_rows(rows_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0>, a, threads, s);
+            });
+        });
     });
 }
 
@@ -202,9 +545,37 @@ extern "C" int stdmlc_distill_backward(const stdmlc_distill *d, int device, void
         check(d);
         if (d->rows == 0) { return; }
         require(d->dloss != nullptr && d->dlogits != nullptr, "distill_loss: null operand");
+        Args a{*d, nullptr, nullptr, 0, d->dlogits, 1};
+        int threads;
+        launch_shape(*d, a.cluster, threads);
         by_dtype(d->dt, [&](auto t) {
-            grad_kernel<decltype(t)><<<static_cast<unsigned int>(d->rows), kThreads, 8 * d->top_count,
-                                       static_cast<cudaStream_t>(stream)>>>(*d);
+            by_need(*d, [&](auto hard, auto soft) {
+                launch_rows(grad_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0>, a, threads,
+                            static_cast<cudaStream_t>(stream));
+            });
         });
     });
+}
+
+extern "C" int stdmlc_distill_scale(void *grad, long long count, int dt, const float *by, int device, void *stream)
+{
+    return entry(device, [&] {
+        require(float_type(dt) && count >= 0, "distill_loss: bf16, f16 or f32 expected");
+        if (count == 0) { return; }
+        require(by != nullptr && grad != nullptr && reinterpret_cast<uintptr_t>(grad) % 16 == 0,
+                "distill_loss: a gradient on a 16-byte boundary expected");
+        by_dtype(dt, [&](auto t) {
+            using T = decltype(t);
+            const long long blocks = (count * static_cast<long long>(sizeof(T)) + 512 * 16 - 1) / (512 * 16), most = 4 * sm_count();
+            scale_kernel<T><<<static_cast<unsigned int>(blocks < most ? blocks : most), 512, 0, static_cast<cudaStream_t>(stream)>>>(
+                static_cast<T *>(grad), count, by);
+        });
+    });
+}
+
+extern "C" int stdmlc_stream_capturing(void *stream)
+{
+    cudaStreamCaptureStatus how = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &how) != cudaSuccess) { (void)cudaGetLastError(); }
+    return how != cudaStreamCaptureStatusNone ? 1 : 0;
 }
