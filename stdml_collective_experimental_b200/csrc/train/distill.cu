@@ -139,7 +139,20 @@ struct Running {
     }
 };
 
-template <typename T, bool kHard, bool kSoft>
+// exp(x / t) and exp(x).  kPower: t where it is 1, 2 or 4, so that the one is a power of the other (0: another t); the
+// exponential unit takes 8 cycles for what the others do in one.
+template <bool kHard, bool kSoft, int kPower>
+__device__ __forceinline__ void exponentials(float x, float c, float &hard, float &soft)
+{
+    if constexpr (kSoft) { soft = fast_exp2(x * c); }
+    if constexpr (kHard && kSoft && kPower != 0) {
+        hard = kPower == 1 ? soft : kPower == 2 ? soft * soft : (soft * soft) * (soft * soft);
+    } else if constexpr (kHard) {
+        hard = fast_exp2(x * kLog2E);
+    }
+}
+
+template <typename T, bool kHard, bool kSoft, int kPower>
 struct Walk {
     Running &r;
     float c;  // log2(e) / t
@@ -163,13 +176,14 @@ struct Walk {
     __device__ __forceinline__ void add(float v)
     {
         // (the difference first: a product of its own could overflow at a mask's lowest value)
-        const float below = v - r.most;
-        if constexpr (kHard) { r.hard += fast_exp2(below * kLog2E); }
-        if constexpr (kSoft) { r.soft += fast_exp2(below * c); }
+        float h = 0, q = 0;
+        exponentials<kHard, kSoft, kPower>(v - r.most, c, h, q);
+        if constexpr (kHard) { r.hard += h; }
+        if constexpr (kSoft) { r.soft += q; }
     }
 };
 
-template <typename T, bool kHard, bool kSoft>
+template <typename T, bool kHard, bool kSoft, int kPower>
 struct Write {
     T *dz;
     float most, hard, soft, c;  // factors of the two exponentials
@@ -177,11 +191,9 @@ struct Write {
 
     __device__ __forceinline__ float grad(float v) const
     {
-        const float below = v - most;
-        float g = 0;
-        if constexpr (kHard) { g += hard * fast_exp2(below * kLog2E); }
-        if constexpr (kSoft) { g += soft * fast_exp2(below * c); }
-        return g;
+        float h = 0, q = 0;
+        exponentials<kHard, kSoft, kPower>(v - most, c, h, q);
+        return kHard && kSoft ? hard * h + soft * q : kHard ? hard * h : soft * q;
     }
     __device__ __forceinline__ void one(long long i, float v) { dz[i] = from_f32<T>(grad(v)); }
     __device__ __forceinline__ void vector(long long i, const uint4 &raw)
@@ -236,32 +248,35 @@ __device__ __forceinline__ float teacher_row(const stdmlc_distill &d, long long 
     return nan ? NAN : m == -INFINITY ? -INFINITY : m + logf(sum);
 }
 
-// Gradients at the classes that teacher or label name, over what the walk has written.  `up`: the row's factor.
-template <typename T, bool kHard, bool kSoft>
-__device__ __forceinline__ void correct(const stdmlc_distill &d, const Write<T, kHard, kSoft> &w, const T *z, long long y, float hard, float soft,
-                                        const float *prob, const int *cls, int lead, int step)
+// Gradients at the classes that teacher or label name, over what the walk has written (by all threads of a block).
+template <typename T, typename Writer>
+__device__ __forceinline__ void correct(const stdmlc_distill &d, const Writer &w, const T *z, long long y, float hard, float soft,
+                                        const float *prob, const int *cls)
 {
     bool y_named = false;
-    for (int j = lead; j < d.top_count; j += step) {
+    for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
         const int k = cls[j];
-        if (k < 0) { continue; }
+        const float v = k >= 0 ? to_f32(z[k]) : 0.f;
         bool again = false;  // a class that is named twice is written once, for both
-        for (int i = 0; i < j; ++i) { again = again || cls[i] == k; }
-        if (again) { continue; }
-        float p = prob[j];
-        for (int i = j + 1; i < d.top_count; ++i) { p += cls[i] == k ? prob[i] : 0.f; }
-        w.dz[k] = from_f32<T>(w.grad(to_f32(z[k])) - soft * p - (k == y ? hard : 0.f));
+        float p = 0;
+#pragma unroll 8
+        for (int i = 0; i < d.top_count; ++i) {
+            const bool same = cls[i] == k;
+            again = again | (same & (i < j));
+            p += same ? prob[i] : 0.f;
+        }
+        y_named = y_named | (k == y);
+        if (k >= 0 && !again) { w.dz[k] = from_f32<T>(w.grad(v) - soft * p - (k == y ? hard : 0.f)); }
     }
-    if (y >= 0 && lead == 0) {
-        for (int j = 0; j < d.top_count; ++j) { y_named = y_named || cls[j] == y; }
-        if (!y_named) { w.dz[y] = from_f32<T>(w.grad(to_f32(z[y])) - hard); }
-    }
+    if (y < 0) { return; }  // (the same for all of them)
+    y_named = __syncthreads_or(y_named ? 1 : 0) != 0;
+    if (threadIdx.x == 0 && !y_named) { w.dz[y] = from_f32<T>(w.grad(to_f32(z[y])) - hard); }
 }
 
 constexpr int kStats = 5;  // of a row: maximum, the two sums, the teacher's log-sum, the row's weight
 
 // A row's gradient from its statistics.  kBlocks: threads of the cluster share it.
-template <typename T, bool kHard, bool kSoft>
+template <typename T, bool kHard, bool kSoft, int kPower>
 __device__ __forceinline__ void write_row(const stdmlc_distill &d, long long r, void *grad, float up, float most, float hard_sum,
                                           float soft_sum, float lp, const float *prob, const int *cls, int part, int parts)
 {
@@ -270,7 +285,7 @@ __device__ __forceinline__ void write_row(const stdmlc_distill &d, long long r, 
     const bool labels = d.labels != nullptr, some = lp != -INFINITY;
     const float hard = labels ? up * d.alpha : 0.f, soft = some ? (labels ? up * (1.f - d.alpha) : up) * d.temperature : 0.f;
     const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0;
-    const Write<T, kHard, kSoft> w{dz, most, hard / hard_sum, soft != 0.f ? soft / soft_sum : 0.f, kLog2E / d.temperature, same};
+    const Write<T, kHard, kSoft, kPower> w{dz, most, hard / hard_sum, soft != 0.f ? soft / soft_sum : 0.f, kLog2E / d.temperature, same};
     Share<T>(z, d.classes, part, parts).each(d.classes, part == 0, part == parts - 1, w);
     if (parts > 1) {
         cluster_sync();
@@ -278,7 +293,7 @@ __device__ __forceinline__ void write_row(const stdmlc_distill &d, long long r, 
         __syncthreads();
     }
     const long long y = labels ? label_at(d, r) : -1;
-    if (part == 0) { correct<T, kHard, kSoft>(d, w, z, y, kHard ? hard : 0.f, kSoft ? soft : 0.f, prob, cls, threadIdx.x, blockDim.x); }
+    if (part == 0) { correct(d, w, z, y, kHard ? hard : 0.f, kSoft ? soft : 0.f, prob, cls); }
 }
 
 template <typename T>
@@ -288,8 +303,8 @@ __device__ __forceinline__ void zero_row(T *dz, long long classes, int part, int
     for (long long i = from + threadIdx.x; i < to; i += blockDim.x) { dz[i] = from_f32<T>(0.f); }
 }
 
-// kHard, kSoft: whether either softmax of the student is needed.
-template <typename T, bool kHard, bool kSoft>
+// kHard, kSoft: whether either softmax of the student is needed.  (Two blocks of 512 threads or four of 256 to an SM.)
+template <typename T, bool kHard, bool kSoft, int kPower>
 __global__ void __launch_bounds__(1024) rows_kernel(Args a)
 {
     extern __shared__ float held[];  // the teacher's probabilities, then their classes
@@ -322,7 +337,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Args a)
         }
         const float c = kLog2E / d.temperature;
         Running run;
-        Share<T>(z, d.classes, part, parts).each(d.classes, part == 0, part == parts - 1, Walk<T, kHard, kSoft>{run, c});
+        Share<T>(z, d.classes, part, parts).each(d.classes, part == 0, part == parts - 1, Walk<T, kHard, kSoft, kPower>{run, c});
         float most = block_max(run.most, slots);
         const bool bad = __syncthreads_or(run.hard != run.hard || run.soft != run.soft ? 1 : 0) != 0;  // (fmaxf drops NaN)
         run.raise(most, c);
@@ -375,7 +390,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Args a)
             }
         }
         __syncthreads();
-        if (a.grad != nullptr) { write_row<T, kHard, kSoft>(d, r, a.grad, weight, most, hard, soft, lp, prob, cls, part, parts); }
+        if (a.grad != nullptr) { write_row<T, kHard, kSoft, kPower>(d, r, a.grad, weight, most, hard, soft, lp, prob, cls, part, parts); }
     }
     // Whoever comes last adds up the rows, in their order.
     if (d.reduction == 0 || part != 0) { return; }
@@ -393,7 +408,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Args a)
     if (threadIdx.x == 0) { *d.loss = static_cast<float>(sum); }
 }
 
-template <typename T, bool kHard, bool kSoft>
+template <typename T, bool kHard, bool kSoft, int kPower>
 __global__ void __launch_bounds__(1024) grad_kernel(Args a)
 {
     extern __shared__ float held[];
@@ -417,7 +432,7 @@ __global__ void __launch_bounds__(1024) grad_kernel(Args a)
         }
         __syncthreads();
     }
-    write_row<T, kHard, kSoft>(d, r, a.grad, up, st[0], st[1], st[2], lp, prob, cls, part, parts);
+    write_row<T, kHard, kSoft, kPower>(d, r, a.grad, up, st[0], st[1], st[2], lp, prob, cls, part, parts);
 }
 
 // A gradient that the forward pass has written, times what came from above: nothing to do for one.
@@ -456,15 +471,17 @@ void check(const stdmlc_distill *d)
 
 // How many blocks share a row, and their threads.
 //   Rows that are fewer than the SMs are spread over clusters, down to 4 KB for each block.
-//   A thread has about kUnroll vectors, in up to 1024 threads: with two such blocks on an SM, rows of 256 KB in
-//   work take 76 MB of the L2's 126.
+//   An SM has 1024 threads of these kernels.  The smaller the blocks, the more rows are in work at a time, some waiting
+//   while others load; but rows in work have to stay in the L2 (126 MB) until they are written: 256 threads up to
+//   64 KB of a row (38 MB in work), 512 up to 256 KB (76 MB), 1024 beyond.
+//   With 1024 throughout, 2048 rows of 61 KB took 245 us, and 4096 of 256 KB 691.
 void launch_shape(const stdmlc_distill &d, int &cluster, int &threads)
 {
-    const long long vectors = (d.classes * element_size(d.dt) + 15) / 16;
+    const long long bytes = d.classes * element_size(d.dt);
     cluster = 1;
-    while (cluster < kMostCluster && d.rows * cluster * 2 <= 2 * sm_count() && vectors / (cluster * 2) >= 256) { cluster *= 2; }
-    threads = 128;
-    while (threads < 1024 && threads * kUnroll * cluster < vectors) { threads *= 2; }
+    while (cluster < kMostCluster && d.rows * cluster * 2 <= 2 * sm_count() && bytes / (cluster * 2) >= 4096) { cluster *= 2; }
+    const long long share = bytes / cluster;
+    threads = share <= 4096 ? 128 : share <= (64 << 10) ? 256 : share <= (256 << 10) ? 512 : 1024;
 }
 
 template <typename F>
@@ -472,11 +489,19 @@ void by_need(const stdmlc_distill &d, F f)
 {
     const bool hard = d.labels != nullptr && d.alpha != 0.f, soft = d.labels == nullptr || d.alpha != 1.f;
     if (hard && soft) {
-        f(Int<1>{}, Int<1>{});
+        if (d.temperature == 1.f) {
+            f(Int<1>{}, Int<1>{}, Int<1>{});
+        } else if (d.temperature == 2.f) {
+            f(Int<1>{}, Int<1>{}, Int<2>{});
+        } else if (d.temperature == 4.f) {
+            f(Int<1>{}, Int<1>{}, Int<4>{});
+        } else {
+            f(Int<1>{}, Int<1>{}, Int<0>{});
+        }
     } else if (hard) {
-        f(Int<1>{}, Int<0>{});
+        f(Int<1>{}, Int<0>{}, Int<0>{});
     } else {
-        f(Int<0>{}, Int<1>{});
+        f(Int<0>{}, Int<1>{}, Int<0>{});
     }
 }
 
@@ -532,8 +557,8 @@ extern "C" int stdmlc_distill_forward(const stdmlc_distill *d, int device, void 
             a.count_blocks = d->reduction == 2 ? used : 0;
         }
         by_dtype(d->dt, [&](auto t) {
-            by_need(*d, [&](auto hard, auto soft) {
-                launch_rows(rows_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0>, a, threads, s);
+            by_need(*d, [&](auto hard, auto soft, auto power) {
+                launch_rows(rows_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0, decltype(power)::value>, a, threads, s);
             });
         });
     });
@@ -549,8 +574,8 @@ extern "C" int stdmlc_distill_backward(const stdmlc_distill *d, int device, void
         int threads;
         launch_shape(*d, a.cluster, threads);
         by_dtype(d->dt, [&](auto t) {
-            by_need(*d, [&](auto hard, auto soft) {
-                launch_rows(grad_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0>, a, threads,
+            by_need(*d, [&](auto hard, auto soft, auto power) {
+                launch_rows(grad_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0, decltype(power)::value>, a, threads,
                             static_cast<cudaStream_t>(stream));
             });
         });
