@@ -115,14 +115,6 @@ struct Share {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4 &raw, float (&v)[16 / sizeof(T)])
-{
-    const T *t = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) { v[i] = to_f32(t[i]); }
-}
-
 constexpr float kLowest = -3.402823466e38f;
 
 // Maximum and sums of what a thread has seen.
@@ -139,45 +131,60 @@ struct Running {
     }
 };
 
-// exp(x / t) and exp(x).  kPower: t where it is 1, 2 or 4, so that the one is a power of the other (0: another t); the
-// exponential unit takes 8 cycles for what the others do in one.
+// (z - M) / t in powers of two: a difference and a product, or for 16-bit logits one multiply-add, where neither product can
+// overflow (a mask's lowest value, as the only one in the row, would).
+template <typename T>
+struct Reach {
+    float most, c, shift;
+    bool fused;
+    __device__ __forceinline__ Reach(float most_, float c_) : most(most_), c(c_), shift(-most_ * c_), fused(sizeof(T) == 2 && fabsf(shift) < 1e30f) {}
+    __device__ __forceinline__ float operator()(float v) const { return fused ? fmaf(v, c, shift) : (v - most) * c; }
+};
+
+// exp((z - M) / t) and exp(z - M).  kPower: t where it is 1, 2 or 4, so that the one is a power of the other (0: another
+// t); the exponential unit takes 8 cycles for what the others do in one.
 template <bool kHard, bool kSoft, int kPower>
-__device__ __forceinline__ void exponentials(float x, float c, float &hard, float &soft)
+__device__ __forceinline__ void exponentials(float x, float t, float &hard, float &soft)
 {
-    if constexpr (kSoft) { soft = fast_exp2(x * c); }
+    if constexpr (kSoft) { soft = fast_exp2(x); }
     if constexpr (kHard && kSoft && kPower != 0) {
         hard = kPower == 1 ? soft : kPower == 2 ? soft * soft : (soft * soft) * (soft * soft);
     } else if constexpr (kHard) {
-        hard = fast_exp2(x * kLog2E);
+        hard = fast_exp2(x * t);
     }
 }
 
 template <typename T, bool kHard, bool kSoft, int kPower>
 struct Walk {
     Running &r;
-    float c;  // log2(e) / t
+    float c, t;  // c: log2(e) / t
 
     __device__ __forceinline__ void one(long long, float v)
     {
         r.raise(v, c);
-        add(v);
+        add(v, Reach<T>(r.most, c));
     }
     __device__ __forceinline__ void vector(long long, const uint4 &raw)
     {
         float v[16 / sizeof(T)];
-        unpack<T>(raw, v);
+        unpack16<T>(raw, v);
         float most = v[0];
 #pragma unroll
         for (int i = 1; i < static_cast<int>(16 / sizeof(T)); ++i) { most = fmaxf(most, v[i]); }
         r.raise(most, c);
+        const Reach<T> x(r.most, c);
+        if (x.fused) {
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) { add(v[i]); }
+            for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) { add(v[i], x); }
+        } else {
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) { add(v[i], x); }
+        }
     }
-    __device__ __forceinline__ void add(float v)
+    __device__ __forceinline__ void add(float v, const Reach<T> &x)
     {
-        // (the difference first: a product of its own could overflow at a mask's lowest value)
         float h = 0, q = 0;
-        exponentials<kHard, kSoft, kPower>(v - r.most, c, h, q);
+        exponentials<kHard, kSoft, kPower>(x(v), t, h, q);
         if constexpr (kHard) { r.hard += h; }
         if constexpr (kSoft) { r.soft += q; }
     }
@@ -186,28 +193,33 @@ struct Walk {
 template <typename T, bool kHard, bool kSoft, int kPower>
 struct Write {
     T *dz;
-    float most, hard, soft, c;  // factors of the two exponentials
-    bool same;                  // the gradient's rows lie on the same boundaries as the logits'
+    float most, hard, soft, c, t;  // factors of the two exponentials; c: log2(e) / t
+    bool same;                     // the gradient's rows lie on the same boundaries as the logits'
 
-    __device__ __forceinline__ float grad(float v) const
+    __device__ __forceinline__ float grad(float v, const Reach<T> &x) const
     {
         float h = 0, q = 0;
-        exponentials<kHard, kSoft, kPower>(v - most, c, h, q);
+        exponentials<kHard, kSoft, kPower>(x(v), t, h, q);
         return kHard && kSoft ? hard * h + soft * q : kHard ? hard * h : soft * q;
     }
-    __device__ __forceinline__ void one(long long i, float v) { dz[i] = from_f32<T>(grad(v)); }
+    __device__ __forceinline__ void one(long long i, float v) { dz[i] = from_f32<T>(grad(v, Reach<T>(most, c))); }
     __device__ __forceinline__ void vector(long long i, const uint4 &raw)
     {
         float v[16 / sizeof(T)];
-        unpack<T>(raw, v);
-        __align__(16) T out[16 / sizeof(T)];
+        unpack16<T>(raw, v);
+        const Reach<T> x(most, c);
+        if (x.fused) {
 #pragma unroll
-        for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k) { out[k] = from_f32<T>(grad(v[k])); }
-        if (same) {
-            __stcs(reinterpret_cast<uint4 *>(dz + i), *reinterpret_cast<const uint4 *>(out));
+            for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k) { v[k] = grad(v[k], x); }
         } else {
 #pragma unroll
-            for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k) { dz[i + k] = out[k]; }
+            for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k) { v[k] = grad(v[k], x); }
+        }
+        if (same) {
+            __stcs(reinterpret_cast<uint4 *>(dz + i), pack16<T>(v));
+        } else {
+#pragma unroll
+            for (int k = 0; k < static_cast<int>(16 / sizeof(T)); ++k) { dz[i + k] = from_f32<T>(v[k]); }
         }
     }
 };
@@ -253,6 +265,7 @@ template <typename T, typename Writer>
 __device__ __forceinline__ void correct(const stdmlc_distill &d, const Writer &w, const T *z, long long y, float hard, float soft,
                                         const float *prob, const int *cls)
 {
+    const Reach<T> x(w.most, w.c);
     bool y_named = false;
     for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
         const int k = cls[j];
@@ -266,11 +279,11 @@ __device__ __forceinline__ void correct(const stdmlc_distill &d, const Writer &w
             p += same ? prob[i] : 0.f;
         }
         y_named = y_named | (k == y);
-        if (k >= 0 && !again) { w.dz[k] = from_f32<T>(w.grad(v) - soft * p - (k == y ? hard : 0.f)); }
+        if (k >= 0 && !again) { w.dz[k] = from_f32<T>(w.grad(v, x) - soft * p - (k == y ? hard : 0.f)); }
     }
     if (y < 0) { return; }  // (the same for all of them)
     y_named = __syncthreads_or(y_named ? 1 : 0) != 0;
-    if (threadIdx.x == 0 && !y_named) { w.dz[y] = from_f32<T>(w.grad(to_f32(z[y])) - hard); }
+    if (threadIdx.x == 0 && !y_named) { w.dz[y] = from_f32<T>(w.grad(to_f32(z[y]), x) - hard); }
 }
 
 constexpr int kStats = 5;  // of a row: maximum, the two sums, the teacher's log-sum, the row's weight
@@ -285,7 +298,7 @@ __device__ __forceinline__ void write_row(const stdmlc_distill &d, long long r, 
     const bool labels = d.labels != nullptr, some = lp != -INFINITY;
     const float hard = labels ? up * d.alpha : 0.f, soft = some ? (labels ? up * (1.f - d.alpha) : up) * d.temperature : 0.f;
     const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0;
-    const Write<T, kHard, kSoft, kPower> w{dz, most, hard / hard_sum, soft != 0.f ? soft / soft_sum : 0.f, kLog2E / d.temperature, same};
+    const Write<T, kHard, kSoft, kPower> w{dz, most, hard / hard_sum, soft != 0.f ? soft / soft_sum : 0.f, kLog2E / d.temperature, d.temperature, same};
     Share<T>(z, d.classes, part, parts).each(d.classes, part == 0, part == parts - 1, w);
     if (parts > 1) {
         cluster_sync();
@@ -337,7 +350,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Args a)
         }
         const float c = kLog2E / d.temperature;
         Running run;
-        Share<T>(z, d.classes, part, parts).each(d.classes, part == 0, part == parts - 1, Walk<T, kHard, kSoft, kPower>{run, c});
+        Share<T>(z, d.classes, part, parts).each(d.classes, part == 0, part == parts - 1, Walk<T, kHard, kSoft, kPower>{run, c, d.temperature});
         float most = block_max(run.most, slots);
         const bool bad = __syncthreads_or(run.hard != run.hard || run.soft != run.soft ? 1 : 0) != 0;  // (fmaxf drops NaN)
         run.raise(most, c);
@@ -445,11 +458,12 @@ __global__ void __launch_bounds__(512) scale_kernel(T *grad, long long many, con
     constexpr int kPer = 16 / sizeof(T);
     uint4 *v = reinterpret_cast<uint4 *>(grad);
     for (long long i = first; i < many / kPer; i += step) {
-        uint4 raw = v[i];
-        T *t = reinterpret_cast<T *>(&raw);
+        const uint4 raw = v[i];
+        float f[kPer];
+        unpack16<T>(raw, f);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) { t[k] = from_f32<T>(to_f32(t[k]) * up); }
-        v[i] = raw;
+        for (int k = 0; k < kPer; ++k) { f[k] *= up; }
+        v[i] = pack16<T>(f);
     }
     for (long long i = many / kPer * kPer + first; i < many; i += step) { grad[i] = from_f32<T>(to_f32(grad[i]) * up); }
 }

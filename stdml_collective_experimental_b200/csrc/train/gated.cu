@@ -46,12 +46,7 @@ __device__ __forceinline__ void put16(unsigned char *mem, int row, int piece, co
 {
     constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < 16 / kPer; ++j) {
-        __align__(16) T t[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) { t[i] = from_f32<T>(v[kPer * j + i]); }
-        *piece_at(mem, row, piece + j) = *reinterpret_cast<const uint4 *>(t);
-    }
+    for (int j = 0; j < 16 / kPer; ++j) { *piece_at(mem, row, piece + j) = pack16<T>(v + kPer * j); }
 }
 
 // Where kPieces pieces of each of 32 rows go, 32 / kPieces rows at a time: to + r * pitch + 16 * piece.
@@ -116,10 +111,10 @@ struct GatedTile {
             constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
             for (int j = 0; j < 16 / kPer; ++j) {
-                __align__(16) T t[kPer];
-                *reinterpret_cast<uint4 *>(t) = reinterpret_cast<const uint4 *>(bias + col)[j];
+                float t[kPer];
+                unpack16<T>(reinterpret_cast<const uint4 *>(bias + col)[j], t);
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) { v[kPer * j + i] += to_f32(t[i]); }
+                for (int i = 0; i < kPer; ++i) { v[kPer * j + i] += t[i]; }
             }
         } else {
 #pragma unroll
@@ -349,6 +344,7 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(GateGrad a)
             if (r + 8 < end) { row.load(a, r + 8, col); }
             constexpr int kSlabs = sizeof(T) == 4 ? kPieces : 1;
             __align__(16) uint16_t out[2][kSlabs][8];
+            float both[2][8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float dh = to_f32(now.dh[i]), g = now.value(now.g, now.low_g, i), u = now.value(now.u, now.low_u, i);
@@ -368,10 +364,13 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(GateGrad a)
 #pragma unroll
                     for (int j = 0; j < kPieces; ++j) { out[1][j][i] = piece[j]; }
                 } else {
-                    const T x = from_f32<T>(dg), y = from_f32<T>(du);
-                    out[0][0][i] = *reinterpret_cast<const uint16_t *>(&x);
-                    out[1][0][i] = *reinterpret_cast<const uint16_t *>(&y);
+                    both[0][i] = dg;
+                    both[1][i] = du;
                 }
+            }
+            if constexpr (sizeof(T) == 2) {
+                *reinterpret_cast<uint4 *>(out[0][0]) = pack16<T>(both[0]);
+                *reinterpret_cast<uint4 *>(out[1][0]) = pack16<T>(both[1]);
             }
             uint16_t *at = a.d + r * a.pitch + col;
 #pragma unroll

@@ -4,6 +4,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cstdint>
+#include <type_traits>
+
 #include "capi_train.h"
 
 namespace stdml::collective::train
@@ -30,6 +33,47 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v)
 {
     return __float2half_rn(v);
+}
+
+// 16 bytes of T from as many values.  (Two at a time: one alone is converted on the unit of the exponential, at an
+// eighth of the rate.)
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16)
+{
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half)
+{
+    const __half2 p = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float *v)
+{
+    if constexpr (sizeof(T) == 4) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    } else {
+        return make_uint4(pack2(v[0], v[1], T{}), pack2(v[2], v[3], T{}), pack2(v[4], v[5], T{}), pack2(v[6], v[7], T{}));
+    }
+}
+// And back.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4 &raw, float *v)
+{
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
 }
 
 // Parameters, of which a kernel reads few: their type is looked up at each access.
