@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Args a)
     __shared__ int counted;
     const stdmlc_distill &d = a.d;
     const int parts = a.cluster, part = parts > 1 ? static_cast<int>(cta_rank()) : 0;
+    if (parts > 1) { cluster_begin(); }
     const long long r = blockIdx.x / parts;
     const T *z = static_cast<const T *>(d.logits) + r * d.logits_row;
     float *prob = held;
@@ -336,6 +337,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(Args a)
     const float lp = teacher_row(d, r, prob, cls, slots);
     const long long y = d.labels != nullptr ? label_at(d, r) : -1;
     const bool counts = d.labels != nullptr ? y >= 0 : lp != -INFINITY;
+    if (parts > 1) { cluster_runs(); }
     if (!counts) {  // (the same in all blocks of the row)
         if (a.grad != nullptr) { zero_row(static_cast<T *>(a.grad) + r * d.classes, d.classes, part, parts); }
         if (part == 0 && threadIdx.x == 0) {

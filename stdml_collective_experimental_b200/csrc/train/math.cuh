@@ -126,7 +126,7 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d)
         a = z;
         d = 1.f;
     } else if constexpr (kAct == STDMLC_ACT_RELU) {
-        a = z > 0.f ? z : (z != z ? z : 0.f);
+        asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(a) : "f"(z));
         d = z > 0.f ? 1.f : 0.f;
     } else if constexpr (kAct == STDMLC_ACT_SILU) {
         const float s = kExact ? 1.f / (1.f + expf(-z)) : fast_rcp(1.f + fast_exp2(-kLog2E * z));

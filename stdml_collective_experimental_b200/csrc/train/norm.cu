@@ -12,7 +12,7 @@ namespace
 Rows rows_of(const stdmlc_rows &r) { return {r.ptr, r.image, r.row}; }
 
 // How the work is cut.
-//   Channels: chunks of whole groups of at most 2048 channels (their sums lie in shared memory), and narrower ones, down to 256
+//   Channels: chunks of whole groups, of at most 2048 channels and 256 groups (their sums lie in shared memory), and narrower ones, down to 256
 //   bytes of a row, while the images' slices alone would leave SMs without work.
 //   Positions: slices of 64 at least, up to eight to a cluster; where clusters would fill less than half of the GPU,
 //   as many slices as it takes and two launches.
@@ -23,7 +23,7 @@ void cut(NormArgs &n, int element)
     n.chunks = 1;
     int per_chunk = n.groups;  // groups
     const auto width = [&] { return per_chunk * n.per; };
-    while (per_chunk > 1 && (width() > 2048 || (n.images * ((n.groups + per_chunk - 1) / per_chunk) * kMostSlices < 2 * sms &&
+    while (per_chunk > 1 && (width() > 2048 || per_chunk > kMostGroups || (n.images * ((n.groups + per_chunk - 1) / per_chunk) * kMostSlices < 2 * sms &&
                                                 width() / 2 * element >= 256 && per_chunk % 2 == 0))) {
         per_chunk = (per_chunk + 1) / 2;
     }

@@ -6,11 +6,13 @@
 //
 // Bytes bound it: images in and out once.  A block takes a slice of an image's positions, of all channels or of a chunk of
 // whole groups; a thread has the same few channels in all its rows, so that sums and factors stay in its registers.
-// Either direction walks its slice twice, first for sums and then for results.  The blocks of an image are a
-// cluster that exchanges its sums through shared memory, and few enough images are in work at a time that the second walk
-// reads from the L2.  Where there are too few images for that to fill the GPU, the two walks are two launches
+// Either direction walks its slice twice, first for sums and then for results; in between, each thread keeps what it has
+// loaded in shared memory, as far as that goes, and loads the rest again.  The blocks of an image are a
+// cluster that exchanges its sums through shared memory.  Where there are too few images for that to fill the GPU, the two walks are two launches
 // of slices of all images, with the sums in memory between them.
 #pragma once
+#include <algorithm>
+
 #include "dispatch.cuh"
 #include "host.hpp"
 #include "ptx.cuh"
@@ -19,6 +21,7 @@ namespace stdml::collective::train
 {
 constexpr int kNormThreads = 512;
 constexpr int kMostSlices = 8;  // of an image, in a cluster
+constexpr int kMostGroups = 256;  // of a chunk
 constexpr int kMostPer = 8192;  // channels of a group
 
 struct Rows {
@@ -36,6 +39,7 @@ struct NormArgs {
     int channels, groups, per, weight_dt;
     int chunks, width;  // of an image's channels: `width` channels in all but the last
     int slices;         // of an image's positions
+    int held;           // rows of a thread that stay in shared memory from the first walk to the second
     int walks;          // 1: first walk alone, 2: second, 3: both, the slices being a cluster
     double eps;
 };
@@ -68,6 +72,12 @@ struct Vec {
     }
 };
 
+// n * i / of, in 32 bits where that does.
+__device__ __forceinline__ long long portion(long long n, int i, int of)
+{
+    return n < (1ll << 27) ? static_cast<unsigned int>(n) * static_cast<unsigned int>(i) / static_cast<unsigned int>(of) : n * i / of;
+}
+
 // What a block works on.
 struct Part {
     long long n;      // image
@@ -77,13 +87,13 @@ struct Part {
 
     __device__ __forceinline__ explicit Part(const NormArgs &a)
     {
-        const int i = blockIdx.x / a.slices;
+        const unsigned int i = blockIdx.x / static_cast<unsigned int>(a.slices);
         slice = blockIdx.x - i * a.slices;
-        n = i / a.chunks;
+        n = i / static_cast<unsigned int>(a.chunks);
         c0 = (i - static_cast<int>(n) * a.chunks) * a.width;
         width = min(a.width, a.channels - c0);
-        from = a.positions * slice / a.slices;
-        to = a.positions * (slice + 1) / a.slices;
+        from = a.slices <= 32 ? portion(a.positions, slice, a.slices) : a.positions * slice / a.slices;
+        to = a.slices <= 32 ? portion(a.positions, slice + 1, a.slices) : a.positions * (slice + 1) / a.slices;
     }
 };
 
@@ -103,11 +113,11 @@ struct Grid {
     __device__ __forceinline__ int row() const { return threadIdx.x / across; }
 };
 
-// The sums of two values for each channel of a block, over its rows of threads: into `total`, in 64 bits.
-// `lines`: blockDim.x * kCh pairs.
+// The sums of two values for each channel of a block, over its rows of threads: into `total`, in 64 bits.  All threads take
+// part: some rows each, then the shares.  `lines`: blockDim.x * kCh pairs; `shares`: blockDim.x pairs.
 template <int kCh>
 __device__ __forceinline__ void column_sums(const Grid<kCh> &g, int pass, int width, const float (&s1)[kCh], const float (&s2)[kCh],
-                                            float2 *lines, double2 *total)
+                                            float2 *lines, double2 *shares, double2 *total)
 {
     __syncthreads();
     const int span = g.across * kCh;
@@ -116,40 +126,119 @@ __device__ __forceinline__ void column_sums(const Grid<kCh> &g, int pass, int wi
         for (int i = 0; i < kCh; ++i) { lines[g.row() * span + (threadIdx.x % g.across) * kCh + i] = make_float2(s1[i], s2[i]); }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < span; c += blockDim.x) {
+    const int helpers = span < kNormThreads ? kNormThreads / span : 1;
+    if (helpers > 1) {
+        const int c = threadIdx.x % span, part = threadIdx.x / span;
+        if (part < helpers) {
+            double a = 0, b = 0;
+            for (int r = part; r < g.down; r += helpers) {
+                const float2 v = lines[r * span + c];
+                a += v.x;
+                b += v.y;
+            }
+            shares[threadIdx.x] = make_double2(a, b);
+        }
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < span; c += kNormThreads) {
         if (pass * span + c >= width) { break; }
         double a = 0, b = 0;
-        for (int r = 0; r < g.down; ++r) {
-            const float2 v = lines[r * span + c];
-            a += v.x;
-            b += v.y;
+        if (helpers > 1) {
+            for (int k = 0; k < helpers; ++k) {
+                a += shares[k * span + c].x;
+                b += shares[k * span + c].y;
+            }
+        } else {
+            for (int r = 0; r < g.down; ++r) {
+                const float2 v = lines[r * span + c];
+                a += v.x;
+                b += v.y;
+            }
         }
         total[pass * span + c] = make_double2(a, b);
     }
 }
 
-// Two doubles of a group at the same place in another block of the cluster.
-__device__ __forceinline__ double2 of_block(const double2 *mine, int block)
+// f(group, first channel's lane, lanes): a thread takes a group of few channels, a warp one of many.  f's values are
+// added up by `gather`.
+constexpr int kFewPer = 16;
+template <typename F>
+__device__ __forceinline__ void each_group(int groups, int per, F f)
+{
+    if (per <= kFewPer) {
+        for (int k = threadIdx.x; k < groups; k += kNormThreads) { f(k, 0, 1, [](double v) { return v; }); }
+    } else {
+        for (int k = threadIdx.x >> 5; k < groups; k += kNormThreads / 32) {
+            f(k, static_cast<int>(threadIdx.x & 31), 32, [](double v) { return warp_sum(v); });
+        }
+    }
+}
+
+// A thread's rows of a matrix, one after the other.
+template <typename V>
+struct Walker {
+    const char *at;
+    long long step;  // bytes to the next row
+
+    template <typename T>
+    __device__ __forceinline__ Walker(const T *image, long long row, long long first, int column, int channels, int down)
+        : at(reinterpret_cast<const char *>(image + first * row + column * channels)), step(static_cast<long long>(sizeof(T)) * row * down)
+    {
+    }
+    __device__ __forceinline__ V load(int k) const { return *reinterpret_cast<const V *>(at + k * step); }
+    __device__ __forceinline__ void store(int k, const V &v) const { *reinterpret_cast<V *>(const_cast<char *>(at) + k * step) = v; }
+    __device__ __forceinline__ void next(int k) { at += k * step; }
+};
+
+// Two doubles to the same place in a block of the cluster.  (Sent, not fetched: eight reads one after the other took 10 us.)
+__device__ __forceinline__ void send(const double2 *place, int block, const double2 &v)
 {
     uint32_t at;
-    double2 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_at(mine)), "r"(block));
-    asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "r"(at) : "memory");
-    return v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_at(place)), "r"(block));
+    asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(at), "d"(v.x), "d"(v.y) : "memory");
+}
+
+// A slice's sums of a group go to all blocks of the image: [slice][group] in shared memory, or in memory for the second launch.
+__device__ __forceinline__ void publish(const NormArgs &a, const Part &p, double2 *all, int groups, int g0, int k, const double2 &v)
+{
+    if (a.walks == 1) {
+        reinterpret_cast<double2 *>(a.sums)[(p.n * a.slices + p.slice) * a.groups + g0 + k] = v;
+    } else if (a.slices == 1) {
+        all[k] = v;
+    } else {
+        for (int i = 0; i < a.slices; ++i) { send(all + p.slice * groups + k, i, v); }
+    }
+}
+__device__ __forceinline__ double2 published(const NormArgs &a, const Part &p, const double2 *all, int groups, int g0, int k, int slice)
+{
+    return a.walks == 2 ? reinterpret_cast<const double2 *>(a.sums)[(p.n * a.slices + slice) * a.groups + g0 + k] : all[slice * groups + k];
 }
 
 // `vector`: how many channels side by side all addresses allow to be read at once.
 void norm_forward_launch(const NormArgs &n, int dt, int vector, int act, cudaStream_t s);
 void norm_backward_launch(const NormArgs &n, int dt, int vector, int act, cudaStream_t s);
 
-// One launch of clusters, or one for each walk.
+// One launch of clusters, or one for each walk.  row_bytes: what a thread keeps of a row.
 template <typename Kernel>
-void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, cudaStream_t s)
+void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, int row_bytes, cudaStream_t s)
 {
     const long long blocks = n.images * n.chunks * n.slices;
-    // lines of sums, totals of channels, sums of groups
-    const size_t smem = sizeof(float2) * kNormThreads * channels_per_thread + sizeof(double2) * (n.width + n.width / n.per);
-    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)), "shared memory");
+    // lines of sums, first values, shares of the lines, totals of channels, sums of groups (of all slices); then what is held
+    const size_t sums = sizeof(float2) * kNormThreads * channels_per_thread + sizeof(float) * ((n.width + 3) / 4 * 4) +
+                        sizeof(double2) * (kNormThreads + n.width + (n.walks == 3 ? n.slices : 1) * (n.width / n.per));
+    size_t held = 0;
+    if (n.walks == 3) {
+        const int columns = (n.width + channels_per_thread - 1) / channels_per_thread;
+        const long long down = columns < kNormThreads ? kNormThreads / columns : 1;
+        const long long rows = (n.positions + n.slices - 1) / n.slices, need = (rows + down - 1) / down;
+        // all of it, or as much as leaves room for two blocks on an SM (one alone, which held all of 196 KB, took twice as
+        // long: nothing is under way while it sums)
+        constexpr size_t kTwo = 113 << 10;
+        const size_t line = static_cast<size_t>(kNormThreads) * row_bytes;
+        n.held = columns > kNormThreads || sums >= kTwo ? 0 : static_cast<int>(std::min<long long>(need, static_cast<long long>((kTwo - sums) / line)));
+        held = n.held * line;
+    }
+    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sums + held)), "shared memory");
     for (int walk : {1, 2}) {
         if (n.walks == 3 && walk == 2) { return; }
         NormArgs args = n;
@@ -157,7 +246,7 @@ void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, cudaStream_t
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(static_cast<unsigned int>(blocks));
         cfg.blockDim = dim3(kNormThreads);
-        cfg.dynamicSmemBytes = smem;
+        cfg.dynamicSmemBytes = sums + held;
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;

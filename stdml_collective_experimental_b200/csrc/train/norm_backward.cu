@@ -8,32 +8,50 @@ namespace
 constexpr int kAhead = 2;  // rows that a thread has on their way
 
 // Factors of a thread's channels (four at most: with eight they would not leave room for two blocks on an SM).
+// z = x * scale + shift [+ r]; below `near` (and what r adds) its sign is in doubt.
 template <int kCh>
 struct Factors {
-    float mean[kCh], rstd[kCh], scale[kCh], bias[kCh];
+    float mean[kCh], scale[kCh], shift[kCh], near[kCh];
 };
 
-// dz of a thread's channels in a row, and (x - mean).
+// dz of a thread's channels in a row, and x - mean.
 template <typename T, int kCh, int kAct>
 __device__ __forceinline__ void grad_z(const NormArgs &a, const Part &p, int col, const Factors<kCh> &f, const double2 *stats,
                                        const Vec<T, kCh> &x, const Vec<T, kCh> &r, const Vec<T, kCh> &dy, float (&dz)[kCh], float (&off)[kCh])
 {
+    constexpr float kDoubt = 4e-6f;  // of the terms that z is made of: some 64 steps of 32 bits
+    float z[kCh];
+    bool doubt = false;
 #pragma unroll
     for (int i = 0; i < kCh; ++i) {
         off[i] = x.at(i) - f.mean[i];
-        dz[i] = dy.at(i);
         if constexpr (kAct != STDMLC_ACT_NONE) {
-            const float add = a.r.ptr != nullptr ? r.at(i) : 0.f;
-            float z = off[i] * f.scale[i] + f.bias[i] + add;
-            if constexpr (kAct == STDMLC_ACT_RELU) {
-                // the derivative jumps at zero: a value that 32 bits leave in doubt is placed in 64
-                if (fabsf(z) <= 1e-5f * ((fabsf(x.at(i)) + fabsf(f.mean[i])) * fabsf(f.scale[i]) + fabsf(f.bias[i]) + fabsf(add))) {
-                    const int c = col * kCh + i;
-                    const double2 st = stats[c / a.per];
-                    z = static_cast<float>((x.at(i) - st.x) * st.y * weight_of(a, p.c0 + c) + f.bias[i] + add);
-                }
+            z[i] = fmaf(x.at(i), f.scale[i], f.shift[i]);
+            float near = f.near[i];
+            if (a.r.ptr != nullptr) {
+                z[i] += r.at(i);
+                if (kAct == STDMLC_ACT_RELU) { near = fmaf(fabsf(r.at(i)), kDoubt, near); }
             }
-            dz[i] *= act_grad<T, kAct>(z);
+            if (kAct == STDMLC_ACT_RELU) { doubt = doubt | (fabsf(z[i]) <= near); }
+        }
+    }
+    if (kAct == STDMLC_ACT_RELU && doubt) {
+        // the derivative of relu jumps at zero: values that 32 bits leave in doubt are placed in 64
+#pragma unroll
+        for (int i = 0; i < kCh; ++i) {
+            const int c = col * kCh + i;
+            const double2 st = stats[c / a.per];
+            const double add = a.r.ptr != nullptr ? r.at(i) : 0.f;
+            z[i] = static_cast<float>((x.at(i) - st.x) * st.y * weight_of(a, p.c0 + c) + bias_of(a, p.c0 + c) + add);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) {
+        dz[i] = dy.at(i);
+        if constexpr (kAct == STDMLC_ACT_RELU) {
+            dz[i] = z[i] > 0.f ? dz[i] : 0.f;
+        } else if constexpr (kAct != STDMLC_ACT_NONE) {
+            dz[i] *= act_grad<T, kAct>(z[i]);
         }
     }
 }
@@ -43,10 +61,13 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
     using V = Vec<T, kCh>;
+    const bool cluster = a.walks == 3 && a.slices > 1;
+    if (cluster) { cluster_begin(); }
     const Part p(a);
     const Grid<kCh> g(p.width);
     float2 *lines = reinterpret_cast<float2 *>(raw);
-    double2 *total = reinterpret_cast<double2 *>(lines + kNormThreads * kCh), *group = total + a.width;
+    double2 *shares = reinterpret_cast<double2 *>(lines + kNormThreads * kCh), *total = shares + kNormThreads, *all = total + a.width;
+    V *held = reinterpret_cast<V *>(all + (a.walks == 3 ? a.slices : 1) * (a.width / a.per)) + 2 * threadIdx.x;  // x, dy; a row 2 * kNormThreads on
     const int groups = p.width / a.per, g0 = p.c0 / a.per;
     const double2 *stats = reinterpret_cast<const double2 *>(a.stats) + p.n * a.groups + g0;
     const T *x = static_cast<const T *>(a.x.ptr) + p.n * a.x.image + p.c0, *dy = static_cast<const T *>(a.dy.ptr) + p.n * a.dy.image + p.c0;
@@ -59,32 +80,63 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
         for (int i = 0; i < kCh; ++i) {
             const int c = col * kCh + i;
             const double2 st = stats[c / a.per];
+            const double k = st.y * weight_of(a, p.c0 + c), bias = bias_of(a, p.c0 + c);
             f.mean[i] = static_cast<float>(st.x);
-            f.rstd[i] = static_cast<float>(st.y);
-            f.scale[i] = static_cast<float>(st.y) * weight_of(a, p.c0 + c);
-            f.bias[i] = bias_of(a, p.c0 + c);
+            f.scale[i] = static_cast<float>(k);
+            f.shift[i] = static_cast<float>(bias - st.x * k);
+            f.near[i] = static_cast<float>(4e-6 * (fabs(st.x * k) + fabs(bias)));
         }
         return f;
     };
-    // All rows of a thread's: what(row, x, residual, dy).
-    const auto walk = [&](int col, auto what) {
-        const auto load = [&](long long s, V &vx, V &vr, V &vd) {
-            vx = *reinterpret_cast<const V *>(x + s * a.x.row + col * kCh);
-            if (kAct != STDMLC_ACT_NONE && r != nullptr) { vr = *reinterpret_cast<const V *>(r + s * a.r.row + col * kCh); }
-            vd = *reinterpret_cast<const V *>(dy + s * a.dy.row + col * kCh);
+    // All rows of a thread's: what(x, residual, dy, which of the rows ahead), then next(how many).
+    const auto walk = [&](int col, bool second, auto what, auto next) {
+        const long long first = p.from + g.row();
+        const int rows = static_cast<int>(max(0ll, (p.to - first + g.down - 1) / g.down));
+        Walker<V> wx(x, a.x.row, first, col, kCh, g.down), wd(dy, a.dy.row, first, col, kCh, g.down), wr = wx;
+        if (r != nullptr) { wr = Walker<V>(r, a.r.row, first, col, kCh, g.down); }
+        const auto load = [&](int it, int k, V &vx, V &vr, V &vd) {
+            V *mine = held + 2 * kNormThreads * (it + k);
+            const bool kept = it + k < a.held;
+            if (second && kept) {
+                vx = mine[0];
+                vd = mine[1];
+            } else {
+                vx = wx.load(k);
+                vd = wd.load(k);
+            }
+            if (kAct != STDMLC_ACT_NONE && r != nullptr) { vr = wr.load(k); }
         };
-        long long s = p.from + g.row();
-        for (; s + (kAhead - 1) * g.down < p.to; s += kAhead * g.down) {
+        const auto keep = [&](int it, const V &vx, const V &vd) {
+            if (!second && it < a.held) {
+                V *mine = held + 2 * kNormThreads * it;
+                mine[0] = vx;
+                mine[1] = vd;
+            }
+        };
+        int it = 0;
+        for (; it + kAhead <= rows; it += kAhead) {
             V vx[kAhead], vr[kAhead], vd[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) { load(s + k * g.down, vx[k], vr[k], vd[k]); }
+            for (int k = 0; k < kAhead; ++k) { load(it, k, vx[k], vr[k], vd[k]); }
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) { what(s + k * g.down, vx[k], vr[k], vd[k]); }
+            for (int k = 0; k < kAhead; ++k) {
+                keep(it + k, vx[k], vd[k]);
+                what(vx[k], vr[k], vd[k], k);
+            }
+            wx.next(kAhead);
+            wd.next(kAhead);
+            wr.next(kAhead);
+            next(kAhead);
         }
-        for (; s < p.to; s += g.down) {
+        for (; it < rows; ++it) {
             V vx, vr, vd;
-            load(s, vx, vr, vd);
-            what(s, vx, vr, vd);
+            load(it, 0, vx, vr, vd);
+            keep(it, vx, vd);
+            what(vx, vr, vd, 0);
+            wx.next(1);
+            wd.next(1);
+            wr.next(1);
+            next(1);
         }
     };
 
@@ -95,18 +147,21 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
             float s1[kCh] = {}, s2[kCh] = {};
             if (col < g.columns && g.row() < g.down) {
                 const Factors<kCh> f = factors(col);
-                walk(col, [&](long long, const V &vx, const V &vr, const V &vd) {
+                const auto add = [&](const V &vx, const V &vr, const V &vd, int) {
                     float dz[kCh], off[kCh];
                     grad_z<T, kCh, kAct>(a, p, col, f, stats, vx, vr, vd, dz, off);
 #pragma unroll
                     for (int i = 0; i < kCh; ++i) {
                         s1[i] += dz[i];
-                        s2[i] += dz[i] * (off[i] * f.rstd[i]);
+                        s2[i] += dz[i] * off[i];
                     }
-                });
+                };
+                walk(col, false, add, [](int) {});
             }
-            column_sums<kCh>(g, pass, p.width, s1, s2, lines, total);
+            column_sums<kCh>(g, pass, p.width, s1, s2, lines, shares, total);
         }
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.width; c += kNormThreads) { total[c].y *= stats[c / a.per].y; }  // off * rstd = xh
         __syncthreads();
         if (a.param_sums != nullptr) {
             float *out = a.param_sums + (p.n * a.slices + p.slice) * 2 * a.channels + p.c0;
@@ -115,21 +170,24 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
                 out[a.channels + c] = static_cast<float>(total[c].y);
             }
         }
-        if (a.dx.ptr == nullptr && a.dr.ptr == nullptr) { return; }  // (all blocks)
-        for (int k = threadIdx.x; k < groups; k += blockDim.x) {
+        if (a.dx.ptr == nullptr && a.dr.ptr == nullptr) {  // (in all blocks)
+            if (cluster) { cluster_runs(); }
+            return;
+        }
+        if (cluster) { cluster_runs(); }
+        each_group(groups, a.per, [&](int k, int lane, int lanes, auto gather) {
             double m1 = 0, m2 = 0;
-            for (int c = k * a.per; c < (k + 1) * a.per; ++c) {
+            for (int c = k * a.per + lane; c < (k + 1) * a.per; c += lanes) {
                 const double w = weight_of(a, p.c0 + c);
                 m1 += w * total[c].x;
                 m2 += w * total[c].y;
             }
-            group[k] = make_double2(m1, m2);
-            if (a.walks == 1) {
-                reinterpret_cast<double2 *>(a.sums)[(p.n * a.slices + p.slice) * a.groups + g0 + k] = group[k];
-            }
-        }
+            m1 = gather(m1);
+            m2 = gather(m2);
+            if (lane == 0) { publish(a, p, all, groups, g0, k, make_double2(m1, m2)); }
+        });
         if (a.walks == 1) { return; }
-        if (a.slices > 1) {
+        if (cluster) {
             cluster_sync();
         } else {
             __syncthreads();
@@ -139,10 +197,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
     const double many = static_cast<double>(a.positions) * a.per;
     for (int k = threadIdx.x; k < groups; k += blockDim.x) {
         double m1 = 0, m2 = 0;
-        const double2 *in_memory = reinterpret_cast<const double2 *>(a.sums) + p.n * a.slices * a.groups + g0 + k;
         for (int i = 0; i < a.slices; ++i) {
-            const double2 v = a.walks == 2 ? in_memory[static_cast<long long>(i) * a.groups]
-                              : a.slices > 1 ? of_block(group + k, i) : group[k];
+            const double2 v = published(a, p, all, groups, g0, k, i);
             m1 += v.x;
             m2 += v.y;
         }
@@ -160,55 +216,64 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
         float c1[kCh], c2[kCh];
 #pragma unroll
         for (int i = 0; i < kCh; ++i) {
-            const double2 m = total[(col * kCh + i) / a.per];
-            c1[i] = f.rstd[i] * static_cast<float>(m.x);
-            c2[i] = f.rstd[i] * f.rstd[i] * static_cast<float>(m.y);
+            const int k = (col * kCh + i) / a.per;
+            const double rstd = stats[k].y;
+            c1[i] = static_cast<float>(-rstd * total[k].x);
+            c2[i] = static_cast<float>(-rstd * rstd * total[k].y);
         }
-        walk(col, [&](long long s, const V &vx, const V &vr, const V &vd) {
+        const long long first = p.from + g.row();
+        Walker<V> wo(dx != nullptr ? dx : dr, dx != nullptr ? a.dx.row : a.dr.row, first, col, kCh, g.down), wr = wo;
+        if (dr != nullptr) { wr = Walker<V>(dr, a.dr.row, first, col, kCh, g.down); }
+        const auto write = [&](const V &vx, const V &vr, const V &vd, int k) {
             float dz[kCh], off[kCh];
             grad_z<T, kCh, kAct>(a, p, col, f, stats, vx, vr, vd, dz, off);
             V o;
             if (dr != nullptr) {
                 o.set(dz);
-                *reinterpret_cast<V *>(dr + s * a.dr.row + col * kCh) = o;
+                wr.store(k, o);
             }
             if (dx != nullptr) {
 #pragma unroll
-                for (int i = 0; i < kCh; ++i) { dz[i] = f.scale[i] * dz[i] - c1[i] - off[i] * c2[i]; }
+                for (int i = 0; i < kCh; ++i) { dz[i] = fmaf(f.scale[i], dz[i], fmaf(off[i], c2[i], c1[i])); }
                 o.set(dz);
-                *reinterpret_cast<V *>(dx + s * a.dx.row + col * kCh) = o;
+                wo.store(k, o);
             }
+        };
+        walk(col, a.walks == 3, write, [&](int k) {
+            wo.next(k);
+            wr.next(k);
         });
     }
-    if (a.walks == 3 && a.slices > 1) { cluster_sync(); }  // (nobody leaves while another reads its sums)
 }
 
-// dweight and dbias: the slices' sums, in their order.
-__global__ void __launch_bounds__(256) params_kernel(const float *sums, long long slices, int channels, void *dweight, void *dbias, int dt)
+// dweight and dbias: the slices' sums, in their order (a warp's lanes take channels side by side, its warps every 32nd slice).
+__global__ void __launch_bounds__(1024) params_kernel(const float *sums, long long slices, int channels, void *dweight, void *dbias, int dt)
 {
-    __shared__ double shares[2][8][32];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+    __shared__ double shares[2][32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     double db = 0, dw = 0;
     if (c < channels) {
-        for (long long i = lane; i < slices; i += 8) {
+#pragma unroll 4
+        for (long long i = warp; i < slices; i += 32) {
             db += sums[2 * i * channels + c];
             dw += sums[(2 * i + 1) * channels + c];
         }
     }
-    shares[0][lane][threadIdx.x & 31] = db;
-    shares[1][lane][threadIdx.x & 31] = dw;
+    shares[0][lane][warp] = db;
+    shares[1][lane][warp] = dw;
     __syncthreads();
-    if (lane > 1 || c >= channels) { return; }
-    double sum = 0;
-    for (int i = 0; i < 8; ++i) { sum += shares[lane][i][threadIdx.x & 31]; }
-    void *out = lane == 0 ? dbias : dweight;
-    if (out != nullptr) { store_any(out, c, dt, static_cast<float>(sum)); }
+    for (int which = 0; which < 2; ++which) {  // a warp adds up a channel
+        const double sum = warp_sum(shares[which][warp][lane]);
+        void *out = which == 0 ? dbias : dweight;
+        const int of = blockIdx.x * 32 + warp;
+        if (lane == 0 && out != nullptr && of < channels) { store_any(out, of, dt, static_cast<float>(sum)); }
+    }
 }
 }  // namespace
 
 void norm_params_launch(const NormArgs &n, void *dweight, void *dbias, cudaStream_t s)
 {
-    params_kernel<<<static_cast<unsigned int>((n.channels + 31) / 32), 256, 0, s>>>(n.param_sums, n.images * n.slices, n.channels, dweight,
+    params_kernel<<<static_cast<unsigned int>((n.channels + 31) / 32), 1024, 0, s>>>(n.param_sums, n.images * n.slices, n.channels, dweight,
                                                                                    dbias, n.weight_dt);
 }
 
@@ -220,11 +285,11 @@ void norm_backward_launch(const NormArgs &n, int dt, int vector, int act, cudaSt
             constexpr int kAct = decltype(k)::value;
             if constexpr (kAct != STDMLC_ACT_GELU_TANH) {
                 if (vector >= 4) {
-                    norm_walks(backward_kernel<T, 4, kAct>, n, 4, s);
+                    norm_walks(backward_kernel<T, 4, kAct>, n, 4, 2 * 4 * static_cast<int>(sizeof(T)), s);
                 } else if (vector >= 2) {
-                    norm_walks(backward_kernel<T, 2, kAct>, n, 2, s);
+                    norm_walks(backward_kernel<T, 2, kAct>, n, 2, 2 * 2 * static_cast<int>(sizeof(T)), s);
                 } else {
-                    norm_walks(backward_kernel<T, 1, kAct>, n, 1, s);
+                    norm_walks(backward_kernel<T, 1, kAct>, n, 1, 2 * 1 * static_cast<int>(sizeof(T)), s);
                 }
             }
         });

@@ -12,10 +12,14 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
     using V = Vec<T, kCh>;
+    const bool cluster = a.walks == 3 && a.slices > 1;
+    if (cluster) { cluster_begin(); }
     const Part p(a);
     const Grid<kCh> g(p.width);
     float2 *lines = reinterpret_cast<float2 *>(raw);
-    double2 *total = reinterpret_cast<double2 *>(lines + kNormThreads * kCh), *group = total + a.width;
+    float *lines_first = reinterpret_cast<float *>(raw) + 2 * kNormThreads * kCh;  // each channel's first value in the slice
+    double2 *shares = reinterpret_cast<double2 *>(lines_first + (a.width + 3) / 4 * 4), *total = shares + kNormThreads, *all = total + a.width;
+    V *held = reinterpret_cast<V *>(all + (a.walks == 3 ? a.slices : 1) * (a.width / a.per)) + threadIdx.x;  // a row kNormThreads on
     const int groups = p.width / a.per, g0 = p.c0 / a.per;
     const long long count = p.to - p.from;
     const T *x = static_cast<const T *>(a.x.ptr) + p.n * a.x.image + p.c0;
@@ -27,56 +31,59 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
             float s1[kCh] = {}, s2[kCh] = {};
             if (col < g.columns && g.row() < g.down && count > 0) {
                 const V base = *reinterpret_cast<const V *>(x + p.from * a.x.row + col * kCh);
-                long long s = p.from + g.row();
-                for (; s + (kAhead - 1) * g.down < p.to; s += kAhead * g.down) {
-                    V v[kAhead];
+                if (g.row() == 0) {
 #pragma unroll
-                    for (int k = 0; k < kAhead; ++k) { v[k] = *reinterpret_cast<const V *>(x + (s + k * g.down) * a.x.row + col * kCh); }
-#pragma unroll
-                    for (int k = 0; k < kAhead; ++k) {
-#pragma unroll
-                        for (int i = 0; i < kCh; ++i) {
-                            const float d = v[k].at(i) - base.at(i);
-                            s1[i] += d;
-                            s2[i] += d * d;
-                        }
-                    }
+                    for (int i = 0; i < kCh; ++i) { lines_first[col * kCh + i] = base.at(i); }
                 }
-                for (; s < p.to; s += g.down) {
-                    const V v = *reinterpret_cast<const V *>(x + s * a.x.row + col * kCh);
+                Walker<V> wx(x, a.x.row, p.from + g.row(), col, kCh, g.down);
+                const int rows = static_cast<int>((count - g.row() + g.down - 1) / g.down);
+                const auto add = [&](const V &v) {
 #pragma unroll
                     for (int i = 0; i < kCh; ++i) {
                         const float d = v.at(i) - base.at(i);
                         s1[i] += d;
                         s2[i] += d * d;
                     }
+                };
+                int it = 0;
+                for (; it + kAhead <= rows; it += kAhead, wx.next(kAhead)) {
+                    V v[kAhead];
+#pragma unroll
+                    for (int k = 0; k < kAhead; ++k) { v[k] = wx.load(k); }
+#pragma unroll
+                    for (int k = 0; k < kAhead; ++k) {
+                        if (it + k < a.held) { held[(it + k) * kNormThreads] = v[k]; }
+                        add(v[k]);
+                    }
+                }
+                for (; it < rows; ++it, wx.next(1)) {
+                    const V v = wx.load(0);
+                    if (it < a.held) { held[it * kNormThreads] = v; }
+                    add(v);
                 }
             }
-            column_sums<kCh>(g, pass, p.width, s1, s2, lines, total);
+            column_sums<kCh>(g, pass, p.width, s1, s2, lines, shares, total);
         }
         __syncthreads();
         // ---- mean and sum of squared deviations of each group in the slice
-        for (int k = threadIdx.x; k < groups; k += blockDim.x) {
+        const double each = count > 0 ? 1.0 / static_cast<double>(count) : 0.0, share = 1.0 / a.per;
+        if (cluster) { cluster_runs(); }
+        each_group(groups, a.per, [&](int k, int lane, int lanes, auto gather) {
+            // (a channel's mean: its first value in the slice, and the mean of what lies above it)
+            const auto mean_of = [&](int c) { return count > 0 ? lines_first[c] + total[c].x * each : 0.0; };
             double mean = 0, dev = 0;
-            if (count > 0) {
-                for (int c = 0; c < a.per; ++c) {
-                    const double2 t = total[k * a.per + c];
-                    mean += to_f32(x[p.from * a.x.row + k * a.per + c]) + t.x / count;
-                }
-                mean /= a.per;
-                for (int c = 0; c < a.per; ++c) {
-                    const double2 t = total[k * a.per + c];
-                    const double off = to_f32(x[p.from * a.x.row + k * a.per + c]) + t.x / count - mean;
-                    dev += t.y - t.x * t.x / count + off * off * count;
-                }
+            for (int c = k * a.per + lane; c < (k + 1) * a.per; c += lanes) { mean += mean_of(c); }
+            mean = gather(mean) * share;
+            for (int c = k * a.per + lane; c < (k + 1) * a.per; c += lanes) {
+                const double2 t = total[c];
+                const double off = mean_of(c) - mean;
+                dev += t.y - t.x * t.x * each + off * off * count;
             }
-            group[k] = make_double2(mean, dev);
-            if (a.walks == 1) {
-                reinterpret_cast<double2 *>(a.sums)[(p.n * a.slices + p.slice) * a.groups + g0 + k] = group[k];
-            }
-        }
+            dev = gather(dev);
+            if (lane == 0) { publish(a, p, all, groups, g0, k, make_double2(mean, dev)); }
+        });
         if (a.walks == 1) { return; }
-        if (a.slices > 1) {
+        if (cluster) {
             cluster_sync();
         } else {
             __syncthreads();
@@ -85,15 +92,14 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
     // ---- of the slices together: total[group] = mean, 1 / deviation
     for (int k = threadIdx.x; k < groups; k += blockDim.x) {
         double mean = 0, dev = 0;
-        const double2 *in_memory = reinterpret_cast<const double2 *>(a.sums) + p.n * a.slices * a.groups + g0 + k;
-        const auto slice_of = [&](int i) {
-            return a.walks == 2 ? in_memory[static_cast<long long>(i) * a.groups] : a.slices > 1 ? of_block(group + k, i) : group[k];
+        const auto rows_in = [&](int i) {
+            return static_cast<double>(a.slices <= 32 ? portion(a.positions, i + 1, a.slices) - portion(a.positions, i, a.slices)
+                                                      : a.positions * (i + 1) / a.slices - a.positions * i / a.slices);
         };
-        const auto rows_in = [&](int i) { return a.positions * (i + 1) / a.slices - a.positions * i / a.slices; };
-        for (int i = 0; i < a.slices; ++i) { mean += slice_of(i).x * rows_in(i); }
-        mean /= a.positions;
+        const double each = 1.0 / static_cast<double>(a.positions);
+        for (int i = 0; i < a.slices; ++i) { mean += published(a, p, all, groups, g0, k, i).x * (rows_in(i) * each); }
         for (int i = 0; i < a.slices; ++i) {
-            const double2 v = slice_of(i);
+            const double2 v = published(a, p, all, groups, g0, k, i);
             dev += v.y + (v.x - mean) * (v.x - mean) * rows_in(i) * a.per;
         }
         const double rstd = 1.0 / sqrt(dev / (static_cast<double>(a.positions) * a.per) + a.eps);
@@ -108,44 +114,55 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
     for (int pass = 0; pass < g.passes; ++pass) {
         const int col = g.column(pass);
         if (col >= g.columns || g.row() >= g.down) { continue; }
-        float scale[kCh], mean[kCh], bias[kCh];
+        // (x - mean) * scale + bias as one multiply-add: either way what is lost is what 32 bits lose of mean * scale
+        float scale[kCh], shift[kCh];
 #pragma unroll
         for (int i = 0; i < kCh; ++i) {
             const int c = col * kCh + i;
             const double2 st = total[c / a.per];
-            mean[i] = static_cast<float>(st.x);
-            scale[i] = static_cast<float>(st.y) * weight_of(a, p.c0 + c);
-            bias[i] = bias_of(a, p.c0 + c);
+            const double k = st.y * weight_of(a, p.c0 + c);
+            scale[i] = static_cast<float>(k);
+            shift[i] = static_cast<float>(bias_of(a, p.c0 + c) - st.x * k);
         }
-        const auto finish = [&](const V &v, const V &res, long long s) {
+        const Walker<V> none(x, 0, 0, 0, 0, 0);
+        Walker<V> wx(x, a.x.row, p.from + g.row(), col, kCh, g.down), wy(y, a.y.row, p.from + g.row(), col, kCh, g.down),
+            wr = r != nullptr ? Walker<V>(r, a.r.row, p.from + g.row(), col, kCh, g.down) : none;
+        const int rows = static_cast<int>(max(0ll, (count - g.row() + g.down - 1) / g.down));
+        const auto finish = [&](const V &v, const V &res, int k) {
             float out[kCh];
 #pragma unroll
             for (int i = 0; i < kCh; ++i) {
-                const float add = r != nullptr ? res.at(i) : 0.f, z = (v.at(i) - mean[i]) * scale[i] + bias[i] + add;
+                float z = fmaf(v.at(i), scale[i], shift[i]);
+                if (r != nullptr) { z += res.at(i); }
                 out[i] = act<T, kAct>(z);
             }
             V o;
             o.set(out);
-            *reinterpret_cast<V *>(y + s * a.y.row + col * kCh) = o;
+            wy.store(k, o);
         };
-        long long s = p.from + g.row();
-        for (; s + (kAhead - 1) * g.down < p.to; s += kAhead * g.down) {
+        int it = 0;
+        for (; it + kAhead <= rows; it += kAhead) {
             V v[kAhead], res[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                v[k] = *reinterpret_cast<const V *>(x + (s + k * g.down) * a.x.row + col * kCh);
-                if (r != nullptr) { res[k] = *reinterpret_cast<const V *>(r + (s + k * g.down) * a.r.row + col * kCh); }
+                v[k] = it + k < a.held ? held[(it + k) * kNormThreads] : wx.load(k);
+                if (r != nullptr) { res[k] = wr.load(k); }
             }
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) { finish(v[k], res[k], s + k * g.down); }
+            for (int k = 0; k < kAhead; ++k) { finish(v[k], res[k], k); }
+            wx.next(kAhead);
+            wy.next(kAhead);
+            wr.next(kAhead);
         }
-        for (; s < p.to; s += g.down) {
+        for (; it < rows; ++it) {
             V res;
-            if (r != nullptr) { res = *reinterpret_cast<const V *>(r + s * a.r.row + col * kCh); }
-            finish(*reinterpret_cast<const V *>(x + s * a.x.row + col * kCh), res, s);
+            if (r != nullptr) { res = wr.load(0); }
+            finish(it < a.held ? held[it * kNormThreads] : wx.load(0), res, 0);
+            wx.next(1);
+            wy.next(1);
+            wr.next(1);
         }
     }
-    if (a.walks == 3 && a.slices > 1) { cluster_sync(); }  // (nobody leaves while another reads its sums)
 }
 }  // namespace
 
@@ -157,11 +174,11 @@ void norm_forward_launch(const NormArgs &n, int dt, int vector, int act, cudaStr
             constexpr int kAct = decltype(k)::value, kFull = 16 / sizeof(T);
             if constexpr (kAct != STDMLC_ACT_GELU_TANH) {
                 if (vector >= kFull) {
-                    norm_walks(forward_kernel<T, kFull, kAct>, n, kFull, s);
+                    norm_walks(forward_kernel<T, kFull, kAct>, n, kFull, kFull * static_cast<int>(sizeof(T)), s);
                 } else if (vector >= 2) {
-                    norm_walks(forward_kernel<T, 2, kAct>, n, 2, s);
+                    norm_walks(forward_kernel<T, 2, kAct>, n, 2, 2 * static_cast<int>(sizeof(T)), s);
                 } else {
-                    norm_walks(forward_kernel<T, 1, kAct>, n, 1, s);
+                    norm_walks(forward_kernel<T, 1, kAct>, n, 1, 1 * static_cast<int>(sizeof(T)), s);
                 }
             }
         });

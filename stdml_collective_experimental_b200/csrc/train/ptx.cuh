@@ -20,6 +20,11 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The two halves of it.  A block's shared memory may be written by the others only once it runs: they arrive as they begin, and
+// wait before they send.
+__device__ __forceinline__ void cluster_begin() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_runs() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // ------------------------------------------------------------ barriers in shared memory
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count)
 {
