@@ -70,6 +70,8 @@ NormArgs checked(const stdmlc_norm *a, bool backward)
     n.weight_dt = a->weight_dt;
     n.eps = a->eps;
     if (any) {
+        n.per_position = 1.0 / static_cast<double>(n.positions);
+        n.per_value = n.per_position / n.per;
         cut(n, element_size(a->dt));
         require(n.images * n.chunks * n.slices < (1ll << 31), "group_norm: too many images");
     }

@@ -6,9 +6,10 @@
 //
 // Bytes bound it: images in and out once.  A block takes a slice of an image's positions, of all channels or of a chunk of
 // whole groups; a thread has the same few channels in all its rows, so that sums and factors stay in its registers.
-// Either direction walks its slice twice, first for sums and then for results; in between, each thread keeps what it has
-// loaded in shared memory, as far as that goes, and loads the rest again.  The blocks of an image are a
-// cluster that exchanges its sums through shared memory.  Where there are too few images for that to fill the GPU, the two walks are two launches
+// Either direction walks its slice twice, first for sums and then for results.  The blocks of an image are a
+// cluster that exchanges its sums through shared memory, and the images in work are few enough for the second walk
+// to find most of its values in the L2.  (Keeping them in shared memory instead took a third longer at its best: too few
+// blocks then share an SM, and nothing is under way while one sums.)  Where there are too few images for that to fill the GPU, the two walks are two launches
 // of slices of all images, with the sums in memory between them.
 #pragma once
 #include <algorithm>
@@ -19,7 +20,7 @@
 
 namespace stdml::collective::train
 {
-constexpr int kNormThreads = 512;
+constexpr int kNormThreads = 256;  // four blocks to an SM: while some sum, others load (with two of 512, a tenth slower)
 constexpr int kMostSlices = 8;  // of an image, in a cluster
 constexpr int kMostGroups = 256;  // of a chunk
 constexpr int kMostPer = 8192;  // channels of a group
@@ -39,9 +40,9 @@ struct NormArgs {
     int channels, groups, per, weight_dt;
     int chunks, width;  // of an image's channels: `width` channels in all but the last
     int slices;         // of an image's positions
-    int held;           // rows of a thread that stay in shared memory from the first walk to the second
     int walks;          // 1: first walk alone, 2: second, 3: both, the slices being a cluster
     double eps;
+    double per_position, per_value;  // 1 / positions, 1 / (positions * channels of a group)
 };
 
 __device__ __forceinline__ float weight_of(const NormArgs &a, int c)
@@ -218,27 +219,15 @@ __device__ __forceinline__ double2 published(const NormArgs &a, const Part &p, c
 void norm_forward_launch(const NormArgs &n, int dt, int vector, int act, cudaStream_t s);
 void norm_backward_launch(const NormArgs &n, int dt, int vector, int act, cudaStream_t s);
 
-// One launch of clusters, or one for each walk.  row_bytes: what a thread keeps of a row.
+// One launch of clusters, or one for each walk.
 template <typename Kernel>
-void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, int row_bytes, cudaStream_t s)
+void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, cudaStream_t s)
 {
     const long long blocks = n.images * n.chunks * n.slices;
-    // lines of sums, first values, shares of the lines, totals of channels, sums of groups (of all slices); then what is held
+    // lines of sums, first values, shares of the lines, totals of channels, sums of groups (of all slices)
     const size_t sums = sizeof(float2) * kNormThreads * channels_per_thread + sizeof(float) * ((n.width + 3) / 4 * 4) +
                         sizeof(double2) * (kNormThreads + n.width + (n.walks == 3 ? n.slices : 1) * (n.width / n.per));
-    size_t held = 0;
-    if (n.walks == 3) {
-        const int columns = (n.width + channels_per_thread - 1) / channels_per_thread;
-        const long long down = columns < kNormThreads ? kNormThreads / columns : 1;
-        const long long rows = (n.positions + n.slices - 1) / n.slices, need = (rows + down - 1) / down;
-        // all of it, or as much as leaves room for two blocks on an SM (one alone, which held all of 196 KB, took twice as
-        // long: nothing is under way while it sums)
-        constexpr size_t kTwo = 113 << 10;
-        const size_t line = static_cast<size_t>(kNormThreads) * row_bytes;
-        n.held = columns > kNormThreads || sums >= kTwo ? 0 : static_cast<int>(std::min<long long>(need, static_cast<long long>((kTwo - sums) / line)));
-        held = n.held * line;
-    }
-    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sums + held)), "shared memory");
+    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sums)), "shared memory");
     for (int walk : {1, 2}) {
         if (n.walks == 3 && walk == 2) { return; }
         NormArgs args = n;
@@ -246,7 +235,7 @@ void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, int row_byte
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(static_cast<unsigned int>(blocks));
         cfg.blockDim = dim3(kNormThreads);
-        cfg.dynamicSmemBytes = sums + held;
+        cfg.dynamicSmemBytes = sums;
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -15,7 +15,13 @@ struct Factors {
 };
 
 // dz of a thread's channels in a row, and x - mean.
-template <typename T, int kCh, int kAct>
+// z where 32 bits leave its sign in doubt.
+__device__ __noinline__ float placed(float x, float add, double mean, double rstd, float w, float b)
+{
+    return static_cast<float>((x - mean) * rstd * w + b + add);
+}
+
+template <typename T, int kCh, int kAct, bool kResidual>
 __device__ __forceinline__ void grad_z(const NormArgs &a, const Part &p, int col, const Factors<kCh> &f, const double2 *stats,
                                        const Vec<T, kCh> &x, const Vec<T, kCh> &r, const Vec<T, kCh> &dy, float (&dz)[kCh], float (&off)[kCh])
 {
@@ -28,7 +34,7 @@ __device__ __forceinline__ void grad_z(const NormArgs &a, const Part &p, int col
         if constexpr (kAct != STDMLC_ACT_NONE) {
             z[i] = fmaf(x.at(i), f.scale[i], f.shift[i]);
             float near = f.near[i];
-            if (a.r.ptr != nullptr) {
+            if (kResidual) {
                 z[i] += r.at(i);
                 if (kAct == STDMLC_ACT_RELU) { near = fmaf(fabsf(r.at(i)), kDoubt, near); }
             }
@@ -41,8 +47,7 @@ __device__ __forceinline__ void grad_z(const NormArgs &a, const Part &p, int col
         for (int i = 0; i < kCh; ++i) {
             const int c = col * kCh + i;
             const double2 st = stats[c / a.per];
-            const double add = a.r.ptr != nullptr ? r.at(i) : 0.f;
-            z[i] = static_cast<float>((x.at(i) - st.x) * st.y * weight_of(a, p.c0 + c) + bias_of(a, p.c0 + c) + add);
+            z[i] = placed(x.at(i), kResidual ? r.at(i) : 0.f, st.x, st.y, weight_of(a, p.c0 + c), bias_of(a, p.c0 + c));
         }
     }
 #pragma unroll
@@ -56,8 +61,8 @@ __device__ __forceinline__ void grad_z(const NormArgs &a, const Part &p, int col
     }
 }
 
-template <typename T, int kCh, int kAct>
-__global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
+template <typename T, int kCh, int kAct, bool kResidual>
+__global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
     using V = Vec<T, kCh>;
@@ -67,12 +72,11 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
     const Grid<kCh> g(p.width);
     float2 *lines = reinterpret_cast<float2 *>(raw);
     double2 *shares = reinterpret_cast<double2 *>(lines + kNormThreads * kCh), *total = shares + kNormThreads, *all = total + a.width;
-    V *held = reinterpret_cast<V *>(all + (a.walks == 3 ? a.slices : 1) * (a.width / a.per)) + 2 * threadIdx.x;  // x, dy; a row 2 * kNormThreads on
     const int groups = p.width / a.per, g0 = p.c0 / a.per;
     const double2 *stats = reinterpret_cast<const double2 *>(a.stats) + p.n * a.groups + g0;
     const T *x = static_cast<const T *>(a.x.ptr) + p.n * a.x.image + p.c0, *dy = static_cast<const T *>(a.dy.ptr) + p.n * a.dy.image + p.c0;
     const T *r = static_cast<const T *>(a.r.ptr);
-    if (r != nullptr) { r += p.n * a.r.image + p.c0; }
+    if (kResidual) { r += p.n * a.r.image + p.c0; }
 
     const auto factors = [&](int col) {
         Factors<kCh> f;
@@ -89,40 +93,23 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
         return f;
     };
     // All rows of a thread's: what(x, residual, dy, which of the rows ahead), then next(how many).
-    const auto walk = [&](int col, bool second, auto what, auto next) {
+    const auto walk = [&](int col, auto what, auto next) {
         const long long first = p.from + g.row();
         const int rows = static_cast<int>(max(0ll, (p.to - first + g.down - 1) / g.down));
         Walker<V> wx(x, a.x.row, first, col, kCh, g.down), wd(dy, a.dy.row, first, col, kCh, g.down), wr = wx;
-        if (r != nullptr) { wr = Walker<V>(r, a.r.row, first, col, kCh, g.down); }
-        const auto load = [&](int it, int k, V &vx, V &vr, V &vd) {
-            V *mine = held + 2 * kNormThreads * (it + k);
-            const bool kept = it + k < a.held;
-            if (second && kept) {
-                vx = mine[0];
-                vd = mine[1];
-            } else {
-                vx = wx.load(k);
-                vd = wd.load(k);
-            }
-            if (kAct != STDMLC_ACT_NONE && r != nullptr) { vr = wr.load(k); }
-        };
-        const auto keep = [&](int it, const V &vx, const V &vd) {
-            if (!second && it < a.held) {
-                V *mine = held + 2 * kNormThreads * it;
-                mine[0] = vx;
-                mine[1] = vd;
-            }
+        if (kResidual) { wr = Walker<V>(r, a.r.row, first, col, kCh, g.down); }
+        const auto load = [&](int k, V &vx, V &vr, V &vd) {
+            vx = wx.load(k);
+            vd = wd.load(k);
+            if (kResidual) { vr = wr.load(k); }
         };
         int it = 0;
         for (; it + kAhead <= rows; it += kAhead) {
             V vx[kAhead], vr[kAhead], vd[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) { load(it, k, vx[k], vr[k], vd[k]); }
+            for (int k = 0; k < kAhead; ++k) { load(k, vx[k], vr[k], vd[k]); }
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                keep(it + k, vx[k], vd[k]);
-                what(vx[k], vr[k], vd[k], k);
-            }
+            for (int k = 0; k < kAhead; ++k) { what(vx[k], vr[k], vd[k], k); }
             wx.next(kAhead);
             wd.next(kAhead);
             wr.next(kAhead);
@@ -130,8 +117,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
         }
         for (; it < rows; ++it) {
             V vx, vr, vd;
-            load(it, 0, vx, vr, vd);
-            keep(it, vx, vd);
+            load(0, vx, vr, vd);
             what(vx, vr, vd, 0);
             wx.next(1);
             wd.next(1);
@@ -149,14 +135,14 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
                 const Factors<kCh> f = factors(col);
                 const auto add = [&](const V &vx, const V &vr, const V &vd, int) {
                     float dz[kCh], off[kCh];
-                    grad_z<T, kCh, kAct>(a, p, col, f, stats, vx, vr, vd, dz, off);
+                    grad_z<T, kCh, kAct, kResidual>(a, p, col, f, stats, vx, vr, vd, dz, off);
 #pragma unroll
                     for (int i = 0; i < kCh; ++i) {
                         s1[i] += dz[i];
                         s2[i] += dz[i] * off[i];
                     }
                 };
-                walk(col, false, add, [](int) {});
+                walk(col, add, [](int) {});
             }
             column_sums<kCh>(g, pass, p.width, s1, s2, lines, shares, total);
         }
@@ -194,7 +180,6 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
         }
     }
     // ---- of the slices together: total[group] = m1, m2
-    const double many = static_cast<double>(a.positions) * a.per;
     for (int k = threadIdx.x; k < groups; k += blockDim.x) {
         double m1 = 0, m2 = 0;
         for (int i = 0; i < a.slices; ++i) {
@@ -202,7 +187,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
             m1 += v.x;
             m2 += v.y;
         }
-        total[k] = make_double2(m1 / many, m2 / many);
+        total[k] = make_double2(m1 * a.per_value, m2 * a.per_value);
     }
     __syncthreads();
     // ---- results
@@ -226,7 +211,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
         if (dr != nullptr) { wr = Walker<V>(dr, a.dr.row, first, col, kCh, g.down); }
         const auto write = [&](const V &vx, const V &vr, const V &vd, int k) {
             float dz[kCh], off[kCh];
-            grad_z<T, kCh, kAct>(a, p, col, f, stats, vx, vr, vd, dz, off);
+            grad_z<T, kCh, kAct, kResidual>(a, p, col, f, stats, vx, vr, vd, dz, off);
             V o;
             if (dr != nullptr) {
                 o.set(dz);
@@ -239,7 +224,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) backward_kernel(NormArgs a)
                 wo.store(k, o);
             }
         };
-        walk(col, a.walks == 3, write, [&](int k) {
+        walk(col, write, [&](int k) {
             wo.next(k);
             wr.next(k);
         });
@@ -269,6 +254,14 @@ __global__ void __launch_bounds__(1024) params_kernel(const float *sums, long lo
         if (lane == 0 && out != nullptr && of < channels) { store_any(out, of, dt, static_cast<float>(sum)); }
     }
 }
+template <typename T, int kCh, int kAct>
+void backward(const NormArgs &n, cudaStream_t s)
+{
+    if constexpr (kAct != STDMLC_ACT_NONE) {
+        if (n.r.ptr != nullptr) { return norm_walks(backward_kernel<T, kCh, kAct, true>, n, kCh, s); }
+    }
+    norm_walks(backward_kernel<T, kCh, kAct, false>, n, kCh, s);
+}
 }  // namespace
 
 void norm_params_launch(const NormArgs &n, void *dweight, void *dbias, cudaStream_t s)
@@ -285,11 +278,11 @@ void norm_backward_launch(const NormArgs &n, int dt, int vector, int act, cudaSt
             constexpr int kAct = decltype(k)::value;
             if constexpr (kAct != STDMLC_ACT_GELU_TANH) {
                 if (vector >= 4) {
-                    norm_walks(backward_kernel<T, 4, kAct>, n, 4, 2 * 4 * static_cast<int>(sizeof(T)), s);
+                    backward<T, 4, kAct>(n, s);
                 } else if (vector >= 2) {
-                    norm_walks(backward_kernel<T, 2, kAct>, n, 2, 2 * 2 * static_cast<int>(sizeof(T)), s);
+                    backward<T, 2, kAct>(n, s);
                 } else {
-                    norm_walks(backward_kernel<T, 1, kAct>, n, 1, 2 * 1 * static_cast<int>(sizeof(T)), s);
+                    backward<T, 1, kAct>(n, s);
                 }
             }
         });

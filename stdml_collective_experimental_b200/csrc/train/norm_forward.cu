@@ -7,8 +7,8 @@ namespace
 {
 constexpr int kAhead = 4;  // rows that a thread has on their way
 
-template <typename T, int kCh, int kAct>
-__global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
+template <typename T, int kCh, int kAct, bool kResidual>
+__global__ void __launch_bounds__(kNormThreads, 4) forward_kernel(NormArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
     using V = Vec<T, kCh>;
@@ -19,9 +19,10 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
     float2 *lines = reinterpret_cast<float2 *>(raw);
     float *lines_first = reinterpret_cast<float *>(raw) + 2 * kNormThreads * kCh;  // each channel's first value in the slice
     double2 *shares = reinterpret_cast<double2 *>(lines_first + (a.width + 3) / 4 * 4), *total = shares + kNormThreads, *all = total + a.width;
-    V *held = reinterpret_cast<V *>(all + (a.walks == 3 ? a.slices : 1) * (a.width / a.per)) + threadIdx.x;  // a row kNormThreads on
     const int groups = p.width / a.per, g0 = p.c0 / a.per;
     const long long count = p.to - p.from;
+    // (here, where the loads below hide what a division in 64 bits takes)
+    const double each = count > 0 ? 1.0 / static_cast<double>(count) : 0.0;
     const T *x = static_cast<const T *>(a.x.ptr) + p.n * a.x.image + p.c0;
 
     if ((a.walks & 1) != 0) {
@@ -52,13 +53,11 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
                     for (int k = 0; k < kAhead; ++k) { v[k] = wx.load(k); }
 #pragma unroll
                     for (int k = 0; k < kAhead; ++k) {
-                        if (it + k < a.held) { held[(it + k) * kNormThreads] = v[k]; }
                         add(v[k]);
                     }
                 }
                 for (; it < rows; ++it, wx.next(1)) {
                     const V v = wx.load(0);
-                    if (it < a.held) { held[it * kNormThreads] = v; }
                     add(v);
                 }
             }
@@ -66,7 +65,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
         }
         __syncthreads();
         // ---- mean and sum of squared deviations of each group in the slice
-        const double each = count > 0 ? 1.0 / static_cast<double>(count) : 0.0, share = 1.0 / a.per;
+        const double share = a.per_value * static_cast<double>(a.positions);
         if (cluster) { cluster_runs(); }
         each_group(groups, a.per, [&](int k, int lane, int lanes, auto gather) {
             // (a channel's mean: its first value in the slice, and the mean of what lies above it)
@@ -96,20 +95,19 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
             return static_cast<double>(a.slices <= 32 ? portion(a.positions, i + 1, a.slices) - portion(a.positions, i, a.slices)
                                                       : a.positions * (i + 1) / a.slices - a.positions * i / a.slices);
         };
-        const double each = 1.0 / static_cast<double>(a.positions);
-        for (int i = 0; i < a.slices; ++i) { mean += published(a, p, all, groups, g0, k, i).x * (rows_in(i) * each); }
+        for (int i = 0; i < a.slices; ++i) { mean += published(a, p, all, groups, g0, k, i).x * (rows_in(i) * a.per_position); }
         for (int i = 0; i < a.slices; ++i) {
             const double2 v = published(a, p, all, groups, g0, k, i);
             dev += v.y + (v.x - mean) * (v.x - mean) * rows_in(i) * a.per;
         }
-        const double rstd = 1.0 / sqrt(dev / (static_cast<double>(a.positions) * a.per) + a.eps);
+        const double rstd = rsqrt(dev * a.per_value + a.eps);
         total[k] = make_double2(mean, rstd);
         if (p.slice == 0) { reinterpret_cast<double2 *>(a.stats)[p.n * a.groups + g0 + k] = total[k]; }
     }
     __syncthreads();
     // ---- results
     const T *r = static_cast<const T *>(a.r.ptr);
-    if (r != nullptr) { r += p.n * a.r.image + p.c0; }
+    if (kResidual) { r += p.n * a.r.image + p.c0; }
     T *y = static_cast<T *>(const_cast<void *>(a.y.ptr)) + p.n * a.y.image + p.c0;
     for (int pass = 0; pass < g.passes; ++pass) {
         const int col = g.column(pass);
@@ -124,16 +122,16 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
             scale[i] = static_cast<float>(k);
             shift[i] = static_cast<float>(bias_of(a, p.c0 + c) - st.x * k);
         }
-        const Walker<V> none(x, 0, 0, 0, 0, 0);
         Walker<V> wx(x, a.x.row, p.from + g.row(), col, kCh, g.down), wy(y, a.y.row, p.from + g.row(), col, kCh, g.down),
-            wr = r != nullptr ? Walker<V>(r, a.r.row, p.from + g.row(), col, kCh, g.down) : none;
+            wr = wy;
+        if (kResidual) { wr = Walker<V>(r, a.r.row, p.from + g.row(), col, kCh, g.down); }
         const int rows = static_cast<int>(max(0ll, (count - g.row() + g.down - 1) / g.down));
         const auto finish = [&](const V &v, const V &res, int k) {
             float out[kCh];
 #pragma unroll
             for (int i = 0; i < kCh; ++i) {
                 float z = fmaf(v.at(i), scale[i], shift[i]);
-                if (r != nullptr) { z += res.at(i); }
+                if (kResidual) { z += res.at(i); }
                 out[i] = act<T, kAct>(z);
             }
             V o;
@@ -145,8 +143,8 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
             V v[kAhead], res[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                v[k] = it + k < a.held ? held[(it + k) * kNormThreads] : wx.load(k);
-                if (r != nullptr) { res[k] = wr.load(k); }
+                v[k] = wx.load(k);
+                if (kResidual) { res[k] = wr.load(k); }
             }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) { finish(v[k], res[k], k); }
@@ -156,12 +154,21 @@ __global__ void __launch_bounds__(kNormThreads, 2) forward_kernel(NormArgs a)
         }
         for (; it < rows; ++it) {
             V res;
-            if (r != nullptr) { res = wr.load(0); }
-            finish(it < a.held ? held[it * kNormThreads] : wx.load(0), res, 0);
+            if (kResidual) { res = wr.load(0); }
+            finish(wx.load(0), res, 0);
             wx.next(1);
             wy.next(1);
             wr.next(1);
         }
+    }
+}
+template <typename T, int kCh, int kAct>
+void forward(const NormArgs &n, cudaStream_t s)
+{
+    if (n.r.ptr != nullptr) {
+        norm_walks(forward_kernel<T, kCh, kAct, true>, n, kCh, s);
+    } else {
+        norm_walks(forward_kernel<T, kCh, kAct, false>, n, kCh, s);
     }
 }
 }  // namespace
@@ -174,11 +181,11 @@ void norm_forward_launch(const NormArgs &n, int dt, int vector, int act, cudaStr
             constexpr int kAct = decltype(k)::value, kFull = 16 / sizeof(T);
             if constexpr (kAct != STDMLC_ACT_GELU_TANH) {
                 if (vector >= kFull) {
-                    norm_walks(forward_kernel<T, kFull, kAct>, n, kFull, kFull * static_cast<int>(sizeof(T)), s);
+                    forward<T, kFull, kAct>(n, s);
                 } else if (vector >= 2) {
-                    norm_walks(forward_kernel<T, 2, kAct>, n, 2, 2 * static_cast<int>(sizeof(T)), s);
+                    forward<T, 2, kAct>(n, s);
                 } else {
-                    norm_walks(forward_kernel<T, 1, kAct>, n, 1, 1 * static_cast<int>(sizeof(T)), s);
+                    forward<T, 1, kAct>(n, s);
                 }
             }
         });
