@@ -189,6 +189,12 @@ struct Walker {
     __device__ __forceinline__ V load(int k) const { return *reinterpret_cast<const V *>(at + k * step); }
     __device__ __forceinline__ void store(int k, const V &v) const { *reinterpret_cast<V *>(const_cast<char *>(at) + k * step) = v; }
     __device__ __forceinline__ void next(int k) { at += k * step; }
+    // From the last of `rows` rows back to the first.
+    __device__ __forceinline__ void turn(int rows)
+    {
+        at += (rows - 1) * step;
+        step = -step;
+    }
 };
 
 // Two doubles to the same place in a block of the cluster.  (Sent, not fetched: eight reads one after the other took 10 us.)

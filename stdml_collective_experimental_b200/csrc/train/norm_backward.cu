@@ -93,11 +93,16 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
         return f;
     };
     // All rows of a thread's: what(x, residual, dy, which of the rows ahead), then next(how many).
-    const auto walk = [&](int col, auto what, auto next) {
+    const auto walk = [&](int col, bool back, auto what, auto next) {
         const long long first = p.from + g.row();
         const int rows = static_cast<int>(max(0ll, (p.to - first + g.down - 1) / g.down));
         Walker<V> wx(x, a.x.row, first, col, kCh, g.down), wd(dy, a.dy.row, first, col, kCh, g.down), wr = wx;
         if (kResidual) { wr = Walker<V>(r, a.r.row, first, col, kCh, g.down); }
+        if (back) {  // (what was read last is in the L2 still)
+            wx.turn(rows);
+            wd.turn(rows);
+            wr.turn(rows);
+        }
         const auto load = [&](int k, V &vx, V &vr, V &vd) {
             vx = wx.load(k);
             vd = wd.load(k);
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
                         s2[i] += dz[i] * off[i];
                     }
                 };
-                walk(col, add, [](int) {});
+                walk(col, false, add, [](int) {});
             }
             column_sums<kCh>(g, pass, p.width, s1, s2, lines, shares, total);
         }
@@ -209,6 +214,9 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
         const long long first = p.from + g.row();
         Walker<V> wo(dx != nullptr ? dx : dr, dx != nullptr ? a.dx.row : a.dr.row, first, col, kCh, g.down), wr = wo;
         if (dr != nullptr) { wr = Walker<V>(dr, a.dr.row, first, col, kCh, g.down); }
+        const int rows = static_cast<int>(max(0ll, (p.to - first + g.down - 1) / g.down));
+        wo.turn(rows);
+        wr.turn(rows);
         const auto write = [&](const V &vx, const V &vr, const V &vd, int k) {
             float dz[kCh], off[kCh];
             grad_z<T, kCh, kAct, kResidual>(a, p, col, f, stats, vx, vr, vd, dz, off);
@@ -224,7 +232,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
                 wo.store(k, o);
             }
         };
-        walk(col, write, [&](int k) {
+        walk(col, true, write, [&](int k) {
             wo.next(k);
             wr.next(k);
         });

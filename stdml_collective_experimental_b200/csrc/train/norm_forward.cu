@@ -126,6 +126,9 @@ __global__ void __launch_bounds__(kNormThreads, 4) forward_kernel(NormArgs a)
             wr = wy;
         if (kResidual) { wr = Walker<V>(r, a.r.row, p.from + g.row(), col, kCh, g.down); }
         const int rows = static_cast<int>(max(0ll, (count - g.row() + g.down - 1) / g.down));
+        wx.turn(rows);  // (what was read last is in the L2 still)
+        wy.turn(rows);
+        wr.turn(rows);
         const auto finish = [&](const V &v, const V &res, int k) {
             float out[kCh];
 #pragma unroll
