@@ -5,7 +5,11 @@ ids of length --seq).
 
     torchrun --nproc-per-node N -m stdml_collective_experimental_b200.benchmarks.resnet50_dp \
         [--model resnet50] [--batch 256] [--seq 128] [--steps 10] [--warmup 3] \
-        [--mode ours|nccl|local|all]
+        [--mode ours|nccl|local|all] [--norm batch|group] [--ffn plain|gated] [--teacher K]
+
+--norm group: ResNet-50 with group normalisation; --ffn gated: BERT with gated feed-forward
+blocks; --teacher K: the loss is distillation from a teacher's K largest logits (synthetic), at
+temperature 2, of the classes, or of BERT's vocabulary at every position.
 
 modes: `ours` = DataParallel of this package (gradients live in the symmetric
 heap, fused in-place all-reduce with the 1/N scale, launched from autograd hooks
@@ -22,7 +26,13 @@ import torch.distributed as dist
 
 from .. import DeviceSession
 from ..models.resnet import ResNet50
+from ..ops import distill_loss
 from ..parallel.ddp import DataParallel
+
+
+def make_teacher(shape, k, dev, g):
+    """(logits, classes) of a synthetic teacher's k largest."""
+    return torch.topk(torch.randn(shape, device=dev, generator=g), k)
 
 
 def make_workload(args, rank, dev):
@@ -30,7 +40,7 @@ def make_workload(args, rank, dev):
     g = torch.Generator(device=dev).manual_seed(100 + rank)
     if args.model in ("resnet50", "vgg16"):
         if args.model == "resnet50":
-            model = ResNet50()
+            model = ResNet50(norm=args.norm)
         else:
             from ..models.vgg import VGG16
             model = VGG16()
@@ -38,17 +48,23 @@ def make_workload(args, rank, dev):
         x = torch.randn(args.batch, 3, 224, 224, device=dev, generator=g).to(
             memory_format=torch.channels_last)
         y = torch.randint(0, 1000, (args.batch,), device=dev, generator=g)
-        return model, x, y, torch.nn.CrossEntropyLoss()
+        if not args.teacher:
+            return model, x, y, torch.nn.CrossEntropyLoss()
+        top, index = make_teacher((args.batch, 1000), args.teacher, dev, g)
+        return model, x, y, lambda out, target: distill_loss(out, top, index, target, temperature=2.0)
     if args.model in ("bert-base", "bert-large"):
         from ..models.bert import bert_base, bert_large
-        model = (bert_base() if args.model == "bert-base" else bert_large()).to(dev)
+        model = (bert_base if args.model == "bert-base" else bert_large)(gated=args.ffn == "gated").to(dev)
         x = torch.randint(0, 30522, (args.batch, args.seq), device=dev, generator=g)
         y = torch.randint(0, 2, (args.batch,), device=dev, generator=g)
 
+        top, index = make_teacher((args.batch, args.seq, 30522), args.teacher, dev, g) if args.teacher else (None, None)
+
         def loss(out, target):  # every parameter takes part: sequence output and pooler
             seq, pooled = out
-            return torch.nn.functional.cross_entropy(pooled[:, :2].float(), target) + \
-                seq.float().pow(2).mean()
+            other = distill_loss(model.vocab_logits(seq), top, index, x, temperature=2.0) if args.teacher \
+                else seq.float().pow(2).mean()
+            return torch.nn.functional.cross_entropy(pooled[:, :2].float(), target) + other
         return model, x, y, loss
     raise SystemExit(f"unknown --model {args.model}")
 
@@ -98,6 +114,8 @@ def run_mode(mode, args, sess, rank, world, dev):
         sess.check()
     out = {"mode": mode, "model": args.model, "n_gpus": world, "batch_per_gpu": args.batch,
            "ms_per_step": ms, "images_per_s": world * args.batch / (ms * 1e-3), "loss": float(loss)}
+    out.update({k: v for k, v in (("norm", args.norm), ("ffn", args.ffn), ("teacher", args.teacher))
+                if v not in ("batch", "plain", 0)})
     if args.model.startswith("bert"):
         out["seq_len"] = args.seq
         out["tokens_per_s"] = world * args.batch * args.seq / (ms * 1e-3)
@@ -117,6 +135,9 @@ def main():
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--buckets", type=int, default=4)
     ap.add_argument("--mode", default="all")
+    ap.add_argument("--norm", default="batch", choices=["batch", "group"])
+    ap.add_argument("--ffn", default="plain", choices=["plain", "gated"])
+    ap.add_argument("--teacher", type=int, default=0)
     args = ap.parse_args()
     rank, world, local = (int(os.environ.get(k, d)) for k, d in
                           (("RANK", 0), ("WORLD_SIZE", 1), ("LOCAL_RANK", 0)))

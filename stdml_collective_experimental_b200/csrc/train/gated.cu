@@ -246,21 +246,55 @@ __device__ __forceinline__ void cut(float v, uint16_t (&piece)[kPieces])
     piece[2] = static_cast<uint16_t>(low >> 16);
 }
 
-// Rows of a pitch that TMA takes; 32-bit values as pieces: [pieces][rows][pitch].
+// Rows of a pitch that TMA takes; 32-bit values as pieces: [pieces][rows][pitch].  A thread takes eight columns (all of them
+// are written, up to the pitch), blockIdx.y an operand.
+struct Packed {
+    const void *from;
+    long long row, rows, cols, pitch;
+    uint16_t *to;
+    bool vec;
+};
+struct Packs {
+    Packed of[3];
+};
+
 template <typename T>
-__global__ void pack_kernel(const T *from, long long from_row, long long rows, long long cols, long long pitch, uint16_t *to)
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs packs)
 {
-    const long long many = rows * cols, step = static_cast<long long>(gridDim.x) * blockDim.x;
-    for (long long e = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; e < many; e += step) {
-        const long long r = e / cols, c = e - r * cols;
-        const T v = from[r * from_row + c];
-        uint16_t *at = to + r * pitch + c;
+    const Packed &p = packs.of[blockIdx.y];
+    const int across = static_cast<int>((p.pitch + 7) / 8);
+    const long long many = p.rows * across, step = static_cast<long long>(gridDim.x) * 256;
+    for (long long e = blockIdx.x * 256ll + threadIdx.x; e < many; e += step) {
+        const long long r = many < (1ll << 31) ? static_cast<unsigned int>(e) / static_cast<unsigned int>(across) : e / across;
+        const long long c = (e - r * across) * 8;
+        const T *from = static_cast<const T *>(p.from) + r * p.row + c;
+        uint16_t *to = p.to + r * p.pitch + c;
         if constexpr (sizeof(T) == 4) {
-            uint16_t piece[kPieces];
-            cut(v, piece);
-            for (int i = 0; i < kPieces; ++i) { at[i * rows * pitch] = piece[i]; }
+            float v[8];
+            if (p.vec && c + 8 <= p.cols) {
+                reinterpret_cast<float4 *>(v)[0] = reinterpret_cast<const float4 *>(from)[0];
+                reinterpret_cast<float4 *>(v)[1] = reinterpret_cast<const float4 *>(from)[1];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { v[i] = c + i < p.cols ? from[i] : 0.f; }
+            }
+            __align__(16) uint16_t out[kPieces][8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                uint16_t piece[kPieces];
+                cut(v[i], piece);
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) { out[k][i] = piece[k]; }
+            }
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                *reinterpret_cast<uint4 *>(to + k * p.rows * p.pitch) = *reinterpret_cast<const uint4 *>(out[k]);
+            }
         } else {
-            *at = *reinterpret_cast<const uint16_t *>(&v);
+            __align__(16) uint16_t out[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { out[i] = c + i < p.cols ? reinterpret_cast<const uint16_t *>(from)[i] : 0; }
+            *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(out);
         }
     }
 }
@@ -548,17 +582,26 @@ struct Operand {
             as = {work.take<uint16_t>(pieces_of(dt) * rows * pitch), rows, cols, pitch, pieces_of(dt)};
         }
     }
-    void pack(cudaStream_t s) const
-    {
-        if (!packed || rows == 0) { return; }
-        const long long blocks = (rows * cols + 255) / 256;
-        by_dtype(dt, [&](auto t) {
-            using T = decltype(t);
-            pack_kernel<T><<<static_cast<unsigned int>(std::min(blocks, 8192ll)), 256, 0, s>>>(
-                static_cast<const T *>(from), row, rows, cols, as.pitch, static_cast<uint16_t *>(const_cast<void *>(as.ptr)));
-        });
-    }
 };
+
+// Those of the operands that have to be, in one launch.
+void pack(std::initializer_list<const Operand *> all, cudaStream_t s)
+{
+    Packs packs{};
+    unsigned int count = 0;
+    long long most = 0;
+    int dt = kF32;
+    for (const Operand *o : all) {
+        if (!o->packed) { continue; }
+        dt = o->dt;
+        packs.of[count++] = {o->from, o->row, o->rows, o->cols, o->as.pitch, static_cast<uint16_t *>(const_cast<void *>(o->as.ptr)),
+                             reinterpret_cast<uintptr_t>(o->from) % 16 == 0 && (o->row * element_size(o->dt)) % 16 == 0};
+        most = std::max(most, o->rows * (o->as.pitch / 8));
+    }
+    if (count == 0) { return; }
+    const unsigned int blocks = static_cast<unsigned int>(std::min((most + 255) / 256, 2048ll));
+    by_dtype(dt, [&](auto t) { pack_kernel<decltype(t)><<<dim3(blocks, count), 256, 0, s>>>(packs); });
+}
 
 struct Operands {
     Bump work;
@@ -855,9 +898,7 @@ void forward(const stdmlc_gated *a, cudaStream_t s)
         return;
     }
     Forward f(a);
-    f.x.pack(s);
-    f.w_gate.pack(s);
-    f.w_up.pack(s);
+    pack({&f.x, &f.w_gate, &f.w_up}, s);
     Product &p = f.w.product[0];
     p.a = f.x.as.map(map_type(a->dt), kTileM);
     p.b[0] = f.w_gate.as.map(map_type(a->dt), f.width / kCtas);
@@ -896,10 +937,15 @@ void backward(const stdmlc_gated *a, cudaStream_t s)
                 b.partial, row_blocks(a), a->ffn, a->db_gate, a->db_up, a->dt);
         }
         if (b.w.products == 0) { return; }
+        if (b.dx >= 0 && b.dw >= 0) {
+            pack({&b.x, &b.w_gate, &b.w_up}, s);
+        } else if (b.dx >= 0) {
+            pack({&b.w_gate, &b.w_up}, s);
+        } else {
+            pack({&b.x}, s);
+        }
         PlainTile<T> tile{{{nullptr, nullptr}, {nullptr, nullptr}}, true};
         if (b.dx >= 0) {
-            b.w_gate.pack(s);
-            b.w_up.pack(s);
             Product &p = b.w.product[b.dx];
             p.a = b.d.map(type, kTileM);
             p.b[0] = b.w_gate.as.map(type, kStepK);
@@ -909,7 +955,6 @@ void backward(const stdmlc_gated *a, cudaStream_t s)
             tile.vec = tile.vec && aligned_rows(a->dx, a->hidden, a->dt);
         }
         if (b.dw >= 0) {
-            b.x.pack(s);
             Product &p = b.w.product[b.dw];
             p.a = b.d.map(type, kStepK);
             p.b[0] = b.x.as.map(type, kStepK);
