@@ -17,8 +17,6 @@ namespace stdml::collective::train
 {
 namespace
 {
-constexpr int kPieces = 3;
-
 __device__ unsigned int g_status;
 
 // ------------------------------------------------------------ what the backward pass needs of g and u
@@ -144,7 +142,7 @@ struct GatedTile {
     __device__ __forceinline__ void tile(const Product &p, int, int row0, int nt, int, int slice, unsigned char *mem,
                                          const Source &from) const
     {
-        constexpr int kCols = Saved<T>::kCols, kPasses = Shape<kN>::kBlocks / 2, kPieces = sizeof(T);
+        constexpr int kCols = Saved<T>::kCols, kPasses = Shape<kN, false>::kBlocks / 2, kPieces = sizeof(T);
         const int lane = threadIdx.x & 31;
         const long long first = nt * (kN / 2ll) + kPasses * kCols * slice;
         const RowsOut<kPieces> rows_h(h + first, p.n * static_cast<long long>(sizeof(T)), row0, p.m);
@@ -202,7 +200,7 @@ struct PlainTile {
     __device__ __forceinline__ void tile(const Product &p, int product, int row0, int nt, int z, int slice, unsigned char *mem,
                                          const Source &from) const
     {
-        constexpr int kCols = Shape<kN>::kValues, kBytes = kCols * static_cast<int>(sizeof(T));
+        constexpr int kCols = Shape<kN, false>::kValues, kBytes = kCols * static_cast<int>(sizeof(T));
         static_assert(kBytes <= 128, "one row in shared memory");
         T *to = product == 0 ? (z == 0 ? out[0][0] : out[0][1]) : (z == 0 ? out[1][0] : out[1][1]);
         const long long first = nt * static_cast<long long>(kN) + kCols * slice;
@@ -649,7 +647,7 @@ int columns_of(const Product &p, int width)
 // turn, so the launch lasts for
 //   sum over rounds of C units of the longest of each.
 // A unit lasts for its steps (one of a 256-wide tile takes 0.45 us, which is its way from the L2, and of a 128-wide one
-// 0.75 of that, as its bytes), or for the epilogue of the one before it, which runs beside it; the last epilogue runs alone.  The parts
+// 0.75 of that, as its bytes; of 32-bit operands, six products, 1 us), or for the epilogue of the one before it, which runs beside it; the last epilogue runs alone.  The parts
 // of a tile are written (kWrite steps' time), and read by the last (kRead for each).
 int cut_tiles(Work &w, int clusters, bool wide)
 {
@@ -659,7 +657,7 @@ int cut_tiles(Work &w, int clusters, bool wide)
     int best[3] = {256, 1, 1};
     for (int width : {256, 128}) {
         if (wide && width == 256) { continue; }
-        const double step = width == 256 ? 1.0 : 0.75, area = width / 256.0;
+        const double step = wide ? 2.2 : width == 256 ? 1.0 : 0.75, area = width / 256.0;
         int most[2] = {1, 1};
         long long tiles[2] = {0, 0}, steps[2] = {0, 0};
         for (int q = 0; q < w.products; ++q) {
@@ -677,7 +675,7 @@ int cut_tiles(Work &w, int clusters, bool wide)
                 double main[2] = {0, 0}, after[2] = {0, 0};
                 const int s[2] = {s0, s1};
                 for (int q = 0; q < w.products; ++q) {
-                    main[q] = step * steps[q] * w.pairs / s[q] + kStart;
+                    main[q] = step * steps[q] / s[q] + kStart;
                     after[q] = area * (s[q] > 1 || wide ? kWrite + kRead * s[q] + kEpilogue : kEpilogue);
                 }
                 const long long u0 = tiles[0] * s0, u1 = tiles[1] * s1;
@@ -721,7 +719,7 @@ long long tiles_of(const Product &p) { return static_cast<long long>(p.m_tiles) 
 struct Scratch {
     long long tickets = 0;
 
-    Scratch(Work &w, int clusters, int width, Bump &work)
+    Scratch(Work &w, int clusters, int width, bool wide, Bump &work)
     {
         bool split = false;
         for (int q = 0; q < w.products; ++q) {
@@ -730,7 +728,7 @@ struct Scratch {
         }
         if (!split) { tickets = 0; }
         w.tickets = work.take<unsigned int>(tickets);
-        w.parts = work.take<float>((w.own_part + (w.pairs > 1 ? clusters : 0)) * (width == 256 ? Shape<256>::kPart : Shape<128>::kPart));
+        w.parts = work.take<float>((w.own_part + (wide ? clusters : 0)) * (width == 256 ? Shape<256, false>::kPart : Shape<128, true>::kPart));
     }
     void clear(const Work &w, cudaStream_t s) const
     {
@@ -749,7 +747,7 @@ template <bool kWide, int kN, typename Epilogue>
 void launch_as(const Work &w, const Epilogue &epilogue, int clusters, cudaStream_t s)
 {
     auto kernel = product_kernel<kWide, kN, Epilogue>;
-    constexpr int kSmem = Shape<kN>::kSmem;
+    constexpr int kSmem = Shape<kN, kWide>::kSmem;
     cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem), "shared memory");
     kernel<<<static_cast<unsigned int>(std::min(w.units, clusters) * kCtas), kProductThreads, kSmem, s>>>(w, epilogue);
 }
@@ -808,14 +806,13 @@ struct Forward : Operands {
     Work w{};
     Scratch scratch;
 
-    explicit Forward(const stdmlc_gated *a) : Operands(a), scratch{plan(a), clusters, width, work} {}
+    explicit Forward(const stdmlc_gated *a) : Operands(a), scratch{plan(a), clusters, width, a->dt == kF32, work} {}
 
   private:
     Work &plan(const stdmlc_gated *a)
     {
         w.product[0] = sizes(a->tokens, a->ffn, a->hidden, 1, 1, true);
         w.products = 1;
-        w.pairs = a->dt == kF32 ? 6 : 1;
         w.chunk = kWideChunk;
         width = cut_tiles(w, clusters, a->dt == kF32);
         return w;
@@ -830,7 +827,7 @@ struct Backward : Operands {
     Scratch scratch;
 
     explicit Backward(const stdmlc_gated *a) : Operands(a), d(grads(a)), partial(work.take<float>(2 * row_blocks(a) * a->ffn)),
-          scratch{plan(a), clusters, width, work}
+          scratch{plan(a), clusters, width, a->dt == kF32, work}
     {
     }
 
@@ -856,7 +853,6 @@ struct Backward : Operands {
             if (x && a->dx != nullptr) { w.product[dx = w.products++] = px; }
             if (!x && z > 0) { w.product[dw = w.products++] = pw; }
         }
-        w.pairs = a->dt == kF32 ? 6 : 1;
         w.chunk = kWideChunk;
         if (w.products > 0) { width = cut_tiles(w, clusters, a->dt == kF32); }
         return w;

@@ -21,20 +21,23 @@ constexpr int kSlices = kEpilogueWarps / 4;
 constexpr int kProductThreads = 32 * (4 + kEpilogueWarps);
 constexpr int kStagingBytes = 4096;  // of an epilogue warp: 32 rows of 128 bytes
 
-// What depends on the width of a tile.
-template <int kN>
+// 32-bit operands come in pieces, of which the pairs that reach 2^-24 of the largest are multiplied, smallest first.
+constexpr int kPieces = 3, kPairs = 6;
+__device__ constexpr int kPairA[kPairs] = {0, 2, 1, 0, 1, 0}, kPairB[kPairs] = {2, 0, 1, 1, 0, 0};
+
+// What depends on the width of a tile, and on the operands (kWide: in pieces, of which a stage has all).
+template <int kN, bool kWide>
 struct Shape {
-    static constexpr int kChunkB = kN / kCtas * 128;
-    static constexpr int kStageBytes = kChunkA + kChunkB;
-    static constexpr int kStages = kN == 256 ? 5 : 6;
+    static constexpr int kChunkB = kN / kCtas * 128, kOf = kWide ? kPieces : 1;
+    static constexpr int kStageBytes = kOf * (kChunkA + kChunkB);
+    static constexpr int kStages = kWide ? 2 : kN == 256 ? 5 : 6;
     static constexpr int kSmem = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024 /* alignment */ + 256 /* barriers */;
     static constexpr int kValues = kN / kSlices;  // of a tile that an epilogue thread takes
     static constexpr int kBlocks = kValues / 16;
     static constexpr long long kPart = static_cast<long long>(kCtas) * kEpilogueWarps * 32 * kValues;  // values of a part
 };
 
-// A result, or several (z) of one shape, as sums of products over a reduction.  32-bit operands come in pieces, of
-// which `pairs` products are summed.
+// A result, or several (z) of one shape, as sums of products over a reduction.
 struct Product {
     CUtensorMap a, b[2];
     int across_a, across_b;   // the operand's rows lie along the reduction (it runs across them)
@@ -50,16 +53,13 @@ struct Product {
 
 struct Work {
     Product product[2];
-    int products, units, pairs;
+    int products, units;
     int chunk;          // steps that are summed in tensor memory before 32-bit registers take over (0: all)
     float *parts;       // kPart values for each unit of a split product, then (kWide) for each cluster, from own_part on
     int own_part;
     unsigned int *tickets;  // zero: [tile][CTA of the pair][epilogue warp]
     unsigned int *status;
 };
-
-// The pairs of pieces whose products reach 2^-24 of the largest, smallest first.
-__device__ constexpr signed char kPairA[6] = {0, 2, 1, 0, 1, 0}, kPairB[6] = {2, 0, 1, 1, 0, 0};
 
 // Why a kernel gave up: a wait ran out.
 constexpr unsigned int kWaitRanOut = 1;
@@ -142,7 +142,7 @@ __device__ __forceinline__ Unit unit_at(const Work &w, int i)
 template <int kN>
 __device__ __forceinline__ int block_column(bool two_b, int slice, int block)
 {
-    constexpr int kOf = Shape<kN>::kValues, kHalf = Shape<kN>::kBlocks / 2;
+    constexpr int kOf = Shape<kN, false>::kValues, kHalf = Shape<kN, false>::kBlocks / 2;
     return two_b ? kOf / 2 * slice + 16 * (block % kHalf) + block / kHalf * (kN / 2) : kOf * slice + 16 * block;
 }
 
@@ -179,7 +179,7 @@ struct FromParts {
 #pragma unroll
             for (int i = 0; i < 16; ++i) { v[i] = __ldcg(p + 32 * i); }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { second[i] = __ldcg(p + Shape<kN>::kPart + 32 * i); }
+            for (int i = 0; i < 16; ++i) { second[i] = __ldcg(p + Shape<kN, false>::kPart + 32 * i); }
 #pragma unroll
             for (int i = 0; i < 16; ++i) { v[i] += second[i]; }
             k = 2;
@@ -190,11 +190,11 @@ struct FromParts {
         for (; k < count; k += 2) {
             float first[16], second[16];
             const bool two = k + 1 < count;
-            const float *q = p + k * Shape<kN>::kPart;
+            const float *q = p + k * Shape<kN, false>::kPart;
 #pragma unroll
             for (int i = 0; i < 16; ++i) { first[i] = __ldcg(q + 32 * i); }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { second[i] = two ? __ldcg(q + Shape<kN>::kPart + 32 * i) : 0.f; }
+            for (int i = 0; i < 16; ++i) { second[i] = two ? __ldcg(q + Shape<kN, false>::kPart + 32 * i) : 0.f; }
 #pragma unroll
             for (int i = 0; i < 16; ++i) { v[i] = v[i] + first[i] + second[i]; }
         }
@@ -214,7 +214,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
     extern __shared__ unsigned char raw[];
     __shared__ uint32_t tmem_at;
     __shared__ int dead_flag;
-    using S = Shape<kN>;
+    using S = Shape<kN, kWide>;
     constexpr int kStages = S::kStages, kStageBytes = S::kStageBytes;
     constexpr uint32_t kColumns = 2 * kN;  // of tensor memory: one tile is summed while the other is taken
     unsigned char *ring = raw + ((1024u - (smem_at(raw) & 1023u)) & 1023u);
@@ -245,7 +245,6 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
     tmem_after_sync();
     const uint32_t tmem = tmem_at;
     const int workers = gridDim.x / kCtas, mine = blockIdx.x / kCtas;
-    const int pairs = kWide ? 6 : 1;
 
     if (warp == 0 && lane == 0) {
         // ---- loads
@@ -256,33 +255,29 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
             const Product &p = w.product[u.product];
             const int m0 = u.m + static_cast<int>(rank) * kTileM;
             const int n0 = u.n * (p.two_b ? kN / 2 : kN) + (p.two_b ? 0 : kN / 2 * static_cast<int>(rank));
-            const int chunk = kWide ? w.chunk : u.to - u.from;
-            for (int c = u.from; ok && c < u.to; c += chunk) {
-                for (int pair = 0; ok && pair < pairs; ++pair) {
-                    for (int step = c; step < min(c + chunk, u.to); ++step, ++it) {
-                        const int st = it % kStages;
-                        ok = it < kStages || wait_for(empty + 8 * st, (it / kStages - 1) & 1, dead, w.status);
-                        if (!ok) { break; }
-                        const uint32_t bar = full + 8 * st, at = ring_at + st * kStageBytes;
-                        if (rank == 0) { bar_expect(bar, kCtas * kStageBytes); }
-                        const int second = step >= p.steps ? 1 : 0, k = (step - second * p.steps) * kStepK;
-                        const int a_slab = (kWide ? kPairA[pair] : 0) + second * p.half_slabs + u.z * p.z_slabs;
-                        const int b_slab = kWide ? kPairB[pair] : 0;
-                        const CUtensorMap *b = &p.b[p.two_b ? static_cast<int>(rank) : second];
-                        if (p.across_a) {
-                            box_load<kCtas>(at, &p.a, m0, k, a_slab, bar);
-                            box_load<kCtas>(at + kChunkA / 2, &p.a, m0 + 64, k, a_slab, bar);
-                        } else {
-                            box_load<kCtas>(at, &p.a, k, m0, a_slab, bar);
-                        }
-                        if (p.across_b) {
+            for (int step = u.from; step < u.to; ++step, ++it) {
+                const int st = it % kStages;
+                ok = it < kStages || wait_for(empty + 8 * st, (it / kStages - 1) & 1, dead, w.status);
+                if (!ok) { break; }
+                const uint32_t bar = full + 8 * st, at_a = ring_at + st * kStageBytes, at_b = at_a + S::kOf * kChunkA;
+                if (rank == 0) { bar_expect(bar, kCtas * kStageBytes); }
+                const int second = step >= p.steps ? 1 : 0, k = (step - second * p.steps) * kStepK;
+                const int slab = second * p.half_slabs + u.z * p.z_slabs;
+                const CUtensorMap *b = &p.b[p.two_b ? static_cast<int>(rank) : second];
 #pragma unroll
-                            for (int j = 0; j < kN / kCtas; j += 64) {
-                                box_load<kCtas>(at + kChunkA + 128 * j, b, n0 + j, k, b_slab, bar);
-                            }
-                        } else {
-                            box_load<kCtas>(at + kChunkA, b, k, n0, b_slab, bar);
-                        }
+                for (int piece = 0; piece < S::kOf; ++piece) {
+                    const uint32_t a_to = at_a + piece * kChunkA, b_to = at_b + piece * S::kChunkB;
+                    if (p.across_a) {
+                        box_load<kCtas>(a_to, &p.a, m0, k, slab + piece, bar);
+                        box_load<kCtas>(a_to + kChunkA / 2, &p.a, m0 + 64, k, slab + piece, bar);
+                    } else {
+                        box_load<kCtas>(a_to, &p.a, k, m0, slab + piece, bar);
+                    }
+                    if (p.across_b) {
+#pragma unroll
+                        for (int j = 0; j < kN / kCtas; j += 64) { box_load<kCtas>(b_to + 128 * j, b, n0 + j, k, piece, bar); }
+                    } else {
+                        box_load<kCtas>(b_to, b, k, n0, piece, bar);
                     }
                 }
             }
@@ -309,18 +304,21 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
                 if (!ok) { break; }
                 tmem_after_sync();
                 const uint32_t d = tmem + buf * kN;
-                const int steps = (min(c + chunk, u.to) - c) * pairs;
+                const int steps = min(c + chunk, u.to) - c;
                 for (int k = 0; k < steps; ++k, ++it) {
                     const int st = it % kStages;
                     ok = wait_for(full + 8 * st, (it / kStages) & 1, dead, w.status);
                     if (!ok) { break; }
                     tmem_after_sync();
-                    const uint32_t at = ring_at + st * kStageBytes;
-                    const uint64_t a = operand_desc(at, across_a ? 64 * 128 : 16, 1024);
-                    const uint64_t b = operand_desc(at + kChunkA, across_b ? 64 * 128 : 16, 1024);
+                    const uint32_t at_a = ring_at + st * kStageBytes, at_b = at_a + S::kOf * kChunkA;
 #pragma unroll
-                    for (int j = 0; j < kStepK / 16; ++j) {
-                        mma16<kCtas>(d, a + j * next_a, b + j * next_b, kind, k > 0 || j > 0);
+                    for (int pair = 0; pair < (kWide ? kPairs : 1); ++pair) {
+                        const uint64_t a = operand_desc(at_a + (kWide ? kPairA[pair] * kChunkA : 0), across_a ? 64 * 128 : 16, 1024);
+                        const uint64_t b = operand_desc(at_b + (kWide ? kPairB[pair] * S::kChunkB : 0), across_b ? 64 * 128 : 16, 1024);
+#pragma unroll
+                        for (int j = 0; j < kStepK / 16; ++j) {
+                            mma16<kCtas>(d, a + j * next_a, b + j * next_b, kind, k > 0 || pair > 0 || j > 0);
+                        }
                     }
                     mma_commit<kCtas>(empty + 8 * st);
                 }
