@@ -93,6 +93,7 @@ void done(int rc)
 
 Tensor bytes_like(const Tensor &t, long long n)
 {
+    TORCH_CHECK(n >= 0, stdmlc_last_error());
     return at::empty({n}, t.options().dtype(at::kByte).requires_grad(false).memory_format(std::nullopt));
 }
 

@@ -39,7 +39,8 @@ typedef struct {
     void *workspace;       /* stdmlc_norm_workspace() bytes */
 } stdmlc_norm;
 
-/* How many bytes of workspace a call with these sizes takes; -1: undefined sizes. */
+/* How many bytes of workspace a call with these sizes (and operands and results, as far as they are set) takes on the
+ * current GPU; -1: undefined sizes, or no GPU. */
 long long stdmlc_norm_workspace(const stdmlc_norm *a, int backward);
 int stdmlc_norm_forward(const stdmlc_norm *a, int device, void *stream);
 int stdmlc_norm_backward(const stdmlc_norm *a, int device, void *stream);

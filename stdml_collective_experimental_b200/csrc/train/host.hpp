@@ -71,6 +71,20 @@ int entry(int device, F f)
     }
 }
 
+// The same for a number of bytes: -1 where there is none.
+template <typename F>
+long long bytes_entry(F f)
+{
+    try {
+        return f();
+    } catch (const std::exception &e) {
+        cuda::set_last_error(e.what());
+    } catch (...) {
+        cuda::set_last_error("unknown C++ exception");
+    }
+    return -1;
+}
+
 inline int sm_count()
 {
     int dev = 0, n = 0;

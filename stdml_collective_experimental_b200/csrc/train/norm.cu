@@ -110,8 +110,10 @@ extern "C" long long stdmlc_norm_workspace(const stdmlc_norm *a, int backward)
     n.channels = a->channels;
     n.groups = a->groups;
     n.per = a->channels / a->groups;
-    cut(n, element_size(a->dt));
-    return sums_bytes(n) + (backward != 0 ? 8 * n.images * n.slices * n.channels : 0);
+    return bytes_entry([&] {
+        cut(n, element_size(a->dt));
+        return sums_bytes(n) + (backward != 0 ? 8 * n.images * n.slices * n.channels : 0);
+    });
 }
 
 extern "C" int stdmlc_norm_forward(const stdmlc_norm *a, int device, void *stream)

@@ -233,7 +233,8 @@ void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, cudaStream_t
     // lines of sums, first values, shares of the lines, totals of channels, sums of groups (of all slices)
     const size_t sums = sizeof(float2) * kNormThreads * channels_per_thread + sizeof(float) * ((n.width + 3) / 4 * 4) +
                         sizeof(double2) * (kNormThreads + n.width + (n.walks == 3 ? n.slices : 1) * (n.width / n.per));
-    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sums)), "shared memory");
+    // (the most that any sizes take, always: another thread may be about to launch the same kernel with more)
+    cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10), "shared memory");
     for (int walk : {1, 2}) {
         if (n.walks == 3 && walk == 2) { return; }
         NormArgs args = n;

@@ -236,6 +236,39 @@ def test_group_norm_layouts(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(3, 24, 10, 7), (1, 8, 201, 307)])  # clusters; two launches
+def test_group_norm_gradients_that_nobody_wants(shape):
+    x, res, dy = (channels_last(shape, s, BF16) for s in (1, 2, 3))
+    args = [x, res, rand(shape[1], 4), rand(shape[1], 5)]
+
+    def call(*a):
+        return ops.group_norm(a[0], 4, a[2], a[3], activation="silu", residual=a[1])
+
+    leaves = [t.clone().requires_grad_() for t in args]
+    full = torch.autograd.grad(call(*leaves), leaves, dy)
+    for i in range(4):
+        some = [t.clone().requires_grad_(j == i) for j, t in enumerate(args)]
+        g, = torch.autograd.grad(call(*some), some[i], dy)
+        assert torch.equal(g, full[i])
+    with torch.no_grad():
+        assert torch.equal(call(*leaves), call(*args))
+
+
+@gpu
+@pytest.mark.parametrize("channels,groups", [(5000, 1), (1600, 1600), (8192, 2)])
+def test_group_norm_wide_and_narrow_groups(channels, groups):
+    shape = (2, channels, 3, 5)
+    x, dy = channels_last(shape, 1, F32), channels_last(shape, 2, F32)
+    check_norm(x, groups, rand(channels, 3), rand(channels, 4), 1e-2, "silu", None, dy)
+
+
+@gpu
+def test_group_norm_refuses_the_widest_groups():
+    with pytest.raises(ValueError, match="8192 channels"):
+        ops.group_norm(torch.zeros(1, 8200, 2, 2, device=cuda), 1)
+
+
+@gpu
 @pytest.mark.parametrize("shape", [(0, 8, 3, 3), (2, 8, 0, 3), (0, 8)])
 def test_group_norm_of_nothing(shape):
     x = torch.empty(shape, device=cuda, requires_grad=True)
@@ -726,6 +759,35 @@ def test_on_another_gpu_than_the_current_one():
     assert y.device.index == 1 and torch.cuda.current_device() == 0
     assert torch.equal(y.to(cuda), ops.group_norm(leaves[0], 8, *leaves[1:3], activation="silu", residual=leaves[0]))
     assert len(want) == 7
+
+
+@gpu
+def test_calls_from_several_threads():
+    """Each on a stream of its own, with sizes of its own."""
+    import threading
+    jobs = [a_step(10 * i, dtype) for i, dtype in enumerate((BF16, F32, F16, BF16))]
+    want = [run_step(*job) for job in jobs]
+    torch.cuda.synchronize()
+    got, errors = [None] * len(jobs), []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i] = run_step(*jobs[i])
+                    ops.group_norm(torch.randn(1, 64 * (i + 1), 9, 9, device=cuda), 2 ** i)
+            torch.cuda.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
 
 
 @gpu
