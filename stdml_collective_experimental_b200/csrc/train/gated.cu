@@ -781,7 +781,7 @@ void check(const stdmlc_gated *a)
 
 CUtensorMapDataType map_type(int dt) { return dt == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
 
-// 32-bit sums of pieces are added up in registers after so many steps (two let 1.3e-6 of the gradients go, one 4e-7 or so): the tensor cores cut what they add to a
+// 32-bit sums of pieces are added up in registers after so many steps (one; at two, gradients of 512 x 1024 x 2736 were 1.3e-6 off and not 2.9e-7, for 16 us of 207): the tensor cores cut what they add to a
 // sum of its size, a step of 2^-24 each time, always towards zero.
 constexpr int kWideChunk = 1;
 

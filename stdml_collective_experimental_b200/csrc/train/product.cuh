@@ -238,7 +238,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
         }
         bar_init_visible();
     }
-    if (warp == 2) { tmem_alloc<kCtas>(smem_at(&tmem_at), kColumns); }
+    if (warp == 2) { tmem_alloc(smem_at(&tmem_at), kColumns); }
     tmem_before_sync();
     __syncthreads();
     cluster_sync();
@@ -268,16 +268,16 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
                 for (int piece = 0; piece < S::kOf; ++piece) {
                     const uint32_t a_to = at_a + piece * kChunkA, b_to = at_b + piece * S::kChunkB;
                     if (p.across_a) {
-                        box_load<kCtas>(a_to, &p.a, m0, k, slab + piece, bar);
-                        box_load<kCtas>(a_to + kChunkA / 2, &p.a, m0 + 64, k, slab + piece, bar);
+                        box_load(a_to, &p.a, m0, k, slab + piece, bar);
+                        box_load(a_to + kChunkA / 2, &p.a, m0 + 64, k, slab + piece, bar);
                     } else {
-                        box_load<kCtas>(a_to, &p.a, k, m0, slab + piece, bar);
+                        box_load(a_to, &p.a, k, m0, slab + piece, bar);
                     }
                     if (p.across_b) {
 #pragma unroll
-                        for (int j = 0; j < kN / kCtas; j += 64) { box_load<kCtas>(b_to + 128 * j, b, n0 + j, k, piece, bar); }
+                        for (int j = 0; j < kN / kCtas; j += 64) { box_load(b_to + 128 * j, b, n0 + j, k, piece, bar); }
                     } else {
-                        box_load<kCtas>(b_to, b, k, n0, piece, bar);
+                        box_load(b_to, b, k, n0, piece, bar);
                     }
                 }
             }
@@ -317,12 +317,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
                         const uint64_t b = operand_desc(at_b + (kWide ? kPairB[pair] * S::kChunkB : 0), across_b ? 64 * 128 : 16, 1024);
 #pragma unroll
                         for (int j = 0; j < kStepK / 16; ++j) {
-                            mma16<kCtas>(d, a + j * next_a, b + j * next_b, kind, k > 0 || pair > 0 || j > 0);
+                            mma16(d, a + j * next_a, b + j * next_b, kind, k > 0 || pair > 0 || j > 0);
                         }
                     }
-                    mma_commit<kCtas>(empty + 8 * st);
+                    mma_commit(empty + 8 * st);
                 }
-                if (ok) { mma_commit<kCtas>(summed + 8 * buf); }
+                if (ok) { mma_commit(summed + 8 * buf); }
             }
         }
     } else if (warp >= 4) {
@@ -407,6 +407,6 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
     __syncthreads();
     cluster_sync();
     tmem_after_sync();
-    if (warp == 2) { tmem_free<kCtas>(tmem, kColumns); }
+    if (warp == 2) { tmem_free(tmem, kColumns); }
 }
 }  // namespace stdml::collective::train

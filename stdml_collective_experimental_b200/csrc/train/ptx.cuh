@@ -64,48 +64,25 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity)
 }
 
 // ------------------------------------------------------------ TMA
-__device__ __forceinline__ void map_prefetch(const CUtensorMap *map)
-{
-    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
-// A box at (x, y, z) of a tensor of this GPU; with kCtas == 2 the bytes are counted on the barrier of the
-// pair's first CTA, at the same place.
-template <int kCtas>
+// A box at (x, y, z) of a tensor of this GPU; the bytes are counted on the barrier of the pair's first CTA, at the same
+// place.
 __device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
 {
-    if constexpr (kCtas == 2) {
-        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
-                     "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-                     "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar & 0xFEFFFFFFu)
-                     : "memory");
-    } else {
-        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-                     "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-                     "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-                     : "memory");
-    }
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+                 "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar & 0xFEFFFFFFu)
+                 : "memory");
 }
 
 // ------------------------------------------------------------ tensor memory and products
-template <int kCtas>
 __device__ __forceinline__ void tmem_alloc(uint32_t to, uint32_t columns)
 {
-    if constexpr (kCtas == 2) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-    } else {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
 }
-template <int kCtas>
 __device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns)
 {
-    if constexpr (kCtas == 2) {
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
-    } else {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
-    }
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
 }
 __device__ __forceinline__ void tmem_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -139,38 +116,22 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t at, uint32_t lead, uin
 }
 
 // D (+)= A B over 16 of the reduction; issued by one thread.
-template <int kCtas>
 __device__ __forceinline__ void mma16(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool add)
 {
     const uint32_t on = add ? 1u : 0u;
-    if constexpr (kCtas == 2) {
-        asm volatile("{\n\t"
-                     ".reg .pred p;\n\t"
-                     "setp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
-                     "}" ::"r"(d),
-                     "l"(a), "l"(b), "r"(kind), "r"(on)
-                     : "memory");
-    } else {
-        asm volatile("{\n\t"
-                     ".reg .pred p;\n\t"
-                     "setp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
-                     "}" ::"r"(d),
-                     "l"(a), "l"(b), "r"(kind), "r"(on)
-                     : "memory");
-    }
+    asm volatile("{\n\t"
+                 ".reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+                 "}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(kind), "r"(on)
+                 : "memory");
 }
-// The barrier (of both CTAs of a pair) is arrived at when all products issued so far are done.
-template <int kCtas>
+// The barrier of both CTAs of the pair is arrived at when all products issued so far are done.
 __device__ __forceinline__ void mma_commit(uint32_t bar)
 {
-    if constexpr (kCtas == 2) {
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                     "h"(static_cast<uint16_t>(3))
-                     : "memory");
-    } else {
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-    }
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
 }
 }  // namespace stdml::collective::train
