@@ -114,50 +114,47 @@ struct Grid {
     __device__ __forceinline__ int row() const { return threadIdx.x / across; }
 };
 
-// The sums of two values for each channel of a block, over its rows of threads: into `total`, in 64 bits.  All threads take
-// part: some rows each, then the shares.  `lines`: blockDim.x * kCh pairs; `shares`: blockDim.x pairs.
+// Two sums for each channel of a block, over its rows of threads: into `total`.  A thread adds up few rows in 32 bits, and has the sums of
+// those in 64 here, in `lines`: value i of a thread's channels at line_of(i).  All threads take part in adding them up: some rows
+// each, then the shares.  `shares`: blockDim.x pairs.
+__device__ __forceinline__ int line_of(int i) { return i * kNormThreads + threadIdx.x; }
+
 template <int kCh>
-__device__ __forceinline__ void column_sums(const Grid<kCh> &g, int pass, int width, const float (&s1)[kCh], const float (&s2)[kCh],
-                                            float2 *lines, double2 *shares, double2 *total)
+__device__ __forceinline__ void column_sums(const Grid<kCh> &g, int pass, int width, const double2 *lines, double2 *shares, double2 *total)
 {
     __syncthreads();
-    const int span = g.across * kCh;
-    if (g.row() < g.down) {
-#pragma unroll
-        for (int i = 0; i < kCh; ++i) { lines[g.row() * span + (threadIdx.x % g.across) * kCh + i] = make_float2(s1[i], s2[i]); }
-    }
-    __syncthreads();
+    const int span = g.across * kCh;  // (the first channels of all columns, the second ones, ...)
+    const auto sum_of = [&](int at, int first, int step) {
+        const double2 *line = lines + at / g.across * kNormThreads + at % g.across;
+        double a = 0, b = 0;
+        for (int r = first; r < g.down; r += step) {
+            a += line[r * g.across].x;
+            b += line[r * g.across].y;
+        }
+        return make_double2(a, b);
+    };
     const int helpers = span < kNormThreads ? kNormThreads / span : 1;
     if (helpers > 1) {
-        const int c = threadIdx.x % span, part = threadIdx.x / span;
-        if (part < helpers) {
-            double a = 0, b = 0;
-            for (int r = part; r < g.down; r += helpers) {
-                const float2 v = lines[r * span + c];
-                a += v.x;
-                b += v.y;
-            }
-            shares[threadIdx.x] = make_double2(a, b);
-        }
+        const int part = threadIdx.x / span;
+        if (part < helpers) { shares[threadIdx.x] = sum_of(threadIdx.x % span, part, helpers); }
         __syncthreads();
     }
-    for (int c = threadIdx.x; c < span; c += kNormThreads) {
-        if (pass * span + c >= width) { break; }
-        double a = 0, b = 0;
+    for (int at = threadIdx.x; at < span; at += kNormThreads) {
+        const int c = pass * span + at % g.across * kCh + at / g.across;
+        if (c >= width) { continue; }
+        double2 sum;
         if (helpers > 1) {
+            sum = make_double2(0, 0);
             for (int k = 0; k < helpers; ++k) {
-                a += shares[k * span + c].x;
-                b += shares[k * span + c].y;
+                sum.x += shares[k * span + at].x;
+                sum.y += shares[k * span + at].y;
             }
         } else {
-            for (int r = 0; r < g.down; ++r) {
-                const float2 v = lines[r * span + c];
-                a += v.x;
-                b += v.y;
-            }
+            sum = sum_of(at, 0, 1);
         }
-        total[pass * span + c] = make_double2(a, b);
+        total[c] = sum;
     }
+    __syncthreads();
 }
 
 // f(group, first channel's lane, lanes): a thread takes a group of few channels, a warp one of many.  f's values are
@@ -231,7 +228,7 @@ void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, cudaStream_t
 {
     const long long blocks = n.images * n.chunks * n.slices;
     // lines of sums, first values, shares of the lines, totals of channels, sums of groups (of all slices)
-    const size_t sums = sizeof(float2) * kNormThreads * channels_per_thread + sizeof(float) * ((n.width + 3) / 4 * 4) +
+    const size_t sums = sizeof(double2) * kNormThreads * channels_per_thread + sizeof(float) * ((n.width + 3) / 4 * 4) +
                         sizeof(double2) * (kNormThreads + n.width + (n.walks == 3 ? n.slices : 1) * (n.width / n.per));
     // (the most that any sizes take, always: another thread may be about to launch the same kernel with more)
     cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10), "shared memory");

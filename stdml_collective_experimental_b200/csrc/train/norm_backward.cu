@@ -6,6 +6,7 @@ namespace stdml::collective::train
 namespace
 {
 constexpr int kAhead = 2;  // rows that a thread has on their way
+constexpr int kRun = 64;   // rows whose sums are taken in 32 bits, before 64 take over
 
 // Factors of a thread's channels (four at most: with eight they would not leave room for two blocks on an SM).
 // z = x * scale + shift [+ r]; below `near` (and what r adds) its sign is in doubt.
@@ -70,8 +71,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
     if (cluster) { cluster_begin(); }
     const Part p(a);
     const Grid<kCh> g(p.width);
-    float2 *lines = reinterpret_cast<float2 *>(raw);
-    double2 *shares = reinterpret_cast<double2 *>(lines + kNormThreads * kCh), *total = shares + kNormThreads, *all = total + a.width;
+    double2 *lines = reinterpret_cast<double2 *>(raw), *shares = lines + kNormThreads * kCh, *total = shares + kNormThreads, *all = total + a.width;
     const int groups = p.width / a.per, g0 = p.c0 / a.per;
     const double2 *stats = reinterpret_cast<const double2 *>(a.stats) + p.n * a.groups + g0;
     const T *x = static_cast<const T *>(a.x.ptr) + p.n * a.x.image + p.c0, *dy = static_cast<const T *>(a.dy.ptr) + p.n * a.dy.image + p.c0;
@@ -85,15 +85,16 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
             const int c = col * kCh + i;
             const double2 st = stats[c / a.per];
             const double k = st.y * weight_of(a, p.c0 + c), bias = bias_of(a, p.c0 + c);
+            const float scale = static_cast<float>(k);
             f.mean[i] = static_cast<float>(st.x);
-            f.scale[i] = static_cast<float>(k);
-            f.shift[i] = static_cast<float>(bias - st.x * k);
+            f.scale[i] = scale;
+            f.shift[i] = static_cast<float>(bias - st.x * scale);  // (as in the forward pass)
             f.near[i] = static_cast<float>(4e-6 * (fabs(st.x * k) + fabs(bias)));
         }
         return f;
     };
-    // All rows of a thread's: what(x, residual, dy, which of the rows ahead), then next(how many).
-    const auto walk = [&](int col, bool back, auto what, auto next) {
+    // All rows of a thread's: what(x, residual, dy, which of the rows ahead), then next(how many); pause() after each kRun of them.
+    const auto walk = [&](int col, bool back, auto what, auto next, auto pause) {
         const long long first = p.from + g.row();
         const int rows = static_cast<int>(max(0ll, (p.to - first + g.down - 1) / g.down));
         Walker<V> wx(x, a.x.row, first, col, kCh, g.down), wd(dy, a.dy.row, first, col, kCh, g.down), wr = wx;
@@ -108,19 +109,23 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
             vd = wd.load(k);
             if (kResidual) { vr = wr.load(k); }
         };
-        int it = 0;
-        for (; it + kAhead <= rows; it += kAhead) {
-            V vx[kAhead], vr[kAhead], vd[kAhead];
+        int left = rows;
+        while (left >= kAhead) {
+            const int rest = max(0, left - kRun);
+            for (; left >= rest + kAhead; left -= kAhead) {
+                V vx[kAhead], vr[kAhead], vd[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) { load(k, vx[k], vr[k], vd[k]); }
+                for (int k = 0; k < kAhead; ++k) { load(k, vx[k], vr[k], vd[k]); }
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) { what(vx[k], vr[k], vd[k], k); }
-            wx.next(kAhead);
-            wd.next(kAhead);
-            wr.next(kAhead);
-            next(kAhead);
+                for (int k = 0; k < kAhead; ++k) { what(vx[k], vr[k], vd[k], k); }
+                wx.next(kAhead);
+                wd.next(kAhead);
+                wr.next(kAhead);
+                next(kAhead);
+            }
+            pause();
         }
-        for (; it < rows; ++it) {
+        for (; left > 0; --left) {
             V vx, vr, vd;
             load(0, vx, vr, vd);
             what(vx, vr, vd, 0);
@@ -135,8 +140,18 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
         // ---- sums of dz and of dz * xh
         for (int pass = 0; pass < g.passes; ++pass) {
             const int col = g.column(pass);
-            float s1[kCh] = {}, s2[kCh] = {};
+#pragma unroll
+            for (int i = 0; i < kCh; ++i) { lines[line_of(i)] = make_double2(0, 0); }
             if (col < g.columns && g.row() < g.down) {
+                float s1[kCh] = {}, s2[kCh] = {};
+                const auto keep = [&] {
+#pragma unroll
+                    for (int i = 0; i < kCh; ++i) {
+                        double2 &l = lines[line_of(i)];
+                        l = make_double2(l.x + s1[i], l.y + s2[i]);
+                        s1[i] = s2[i] = 0;
+                    }
+                };
                 const Factors<kCh> f = factors(col);
                 const auto add = [&](const V &vx, const V &vr, const V &vd, int) {
                     float dz[kCh], off[kCh];
@@ -147,11 +162,11 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
                         s2[i] += dz[i] * off[i];
                     }
                 };
-                walk(col, false, add, [](int) {});
+                walk(col, false, add, [](int) {}, keep);
+                keep();
             }
-            column_sums<kCh>(g, pass, p.width, s1, s2, lines, shares, total);
+            column_sums<kCh>(g, pass, p.width, lines, shares, total);
         }
-        __syncthreads();
         for (int c = threadIdx.x; c < p.width; c += kNormThreads) { total[c].y *= stats[c / a.per].y; }  // off * rstd = xh
         __syncthreads();
         if (a.param_sums != nullptr) {
@@ -235,7 +250,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) backward_kernel(NormArgs a)
         walk(col, true, write, [&](int k) {
             wo.next(k);
             wr.next(k);
-        });
+        }, [] {});
     }
 }
 

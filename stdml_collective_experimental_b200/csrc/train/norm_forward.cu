@@ -6,6 +6,40 @@ namespace stdml::collective::train
 namespace
 {
 constexpr int kAhead = 4;  // rows that a thread has on their way
+constexpr int kRun = 16;   // rows whose sums are taken in 32 bits
+
+// Sums of a thread's channels, in 32 bits over a run of rows: of x less a base, and of its square.  s2 - s1^2 / n cancels what the base is
+// off by, so the base is a mean of the thread's own: of the first kAhead rows, which are the first run, and of the last run from then
+// on.  A value that lies D from all others adds D^2 to what is summed, and its run's mean is off by D / 4 at most, so that the next
+// run's 16 squares add up to D^2 before they cancel: 32 bits lose some 2^-21 of D^2 at the worst.  (One base for a whole slice, its first
+// value, was off by D in all of the slice's rows.)
+template <typename T, int kCh>
+struct Run {
+    float base[kCh], s1[kCh] = {}, s2[kCh] = {};
+
+    __device__ __forceinline__ void add(const Vec<T, kCh> &v)
+    {
+#pragma unroll
+        for (int i = 0; i < kCh; ++i) {
+            const float d = v.at(i) - base[i];
+            s1[i] += d;
+            s2[i] += d * d;
+        }
+    }
+    // A run of `rows`: into the sums in 64 bits, of x less `first` (a value of each channel) and of squared deviations from `first`.
+    __device__ __forceinline__ void end(int rows, const float *first, double2 *lines)
+    {
+        const double n = rows, each = rows == kRun ? 1.0 / kRun : rows == kAhead ? 1.0 / kAhead : 1.0 / n;
+#pragma unroll
+        for (int i = 0; i < kCh; ++i) {
+            double2 &l = lines[line_of(i)];
+            const double sum = s1[i], off = static_cast<double>(base[i]) - first[i], mean = off + sum * each;
+            l = make_double2(l.x + n * mean, l.y + (s2[i] - sum * sum * each + n * mean * mean));
+            base[i] += static_cast<float>(sum * each);
+            s1[i] = s2[i] = 0;
+        }
+    }
+};
 
 template <typename T, int kCh, int kAct, bool kResidual>
 __global__ void __launch_bounds__(kNormThreads, 4) forward_kernel(NormArgs a)
@@ -16,8 +50,8 @@ __global__ void __launch_bounds__(kNormThreads, 4) forward_kernel(NormArgs a)
     if (cluster) { cluster_begin(); }
     const Part p(a);
     const Grid<kCh> g(p.width);
-    float2 *lines = reinterpret_cast<float2 *>(raw);
-    float *lines_first = reinterpret_cast<float *>(raw) + 2 * kNormThreads * kCh;  // each channel's first value in the slice
+    double2 *lines = reinterpret_cast<double2 *>(raw);
+    float *lines_first = reinterpret_cast<float *>(lines + kNormThreads * kCh);  // each channel's first value in the slice
     double2 *shares = reinterpret_cast<double2 *>(lines_first + (a.width + 3) / 4 * 4), *total = shares + kNormThreads, *all = total + a.width;
     const int groups = p.width / a.per, g0 = p.c0 / a.per;
     const long long count = p.to - p.from;
@@ -29,41 +63,53 @@ __global__ void __launch_bounds__(kNormThreads, 4) forward_kernel(NormArgs a)
         // ---- sums of x less the slice's first value of the channel, and of their squares
         for (int pass = 0; pass < g.passes; ++pass) {
             const int col = g.column(pass);
-            float s1[kCh] = {}, s2[kCh] = {};
-            if (col < g.columns && g.row() < g.down && count > 0) {
-                const V base = *reinterpret_cast<const V *>(x + p.from * a.x.row + col * kCh);
-                if (g.row() == 0) {
 #pragma unroll
-                    for (int i = 0; i < kCh; ++i) { lines_first[col * kCh + i] = base.at(i); }
-                }
+            for (int i = 0; i < kCh; ++i) { lines[line_of(i)] = make_double2(0, 0); }
+            if (col < g.columns && g.row() == 0 && count > 0) {
+                const V v = *reinterpret_cast<const V *>(x + p.from * a.x.row + col * kCh);
+#pragma unroll
+                for (int i = 0; i < kCh; ++i) { lines_first[col * kCh + i] = v.at(i); }
+            }
+            __syncthreads();
+            if (col < g.columns && g.row() < g.down && count > 0) {
+                const float *first = lines_first + col * kCh;
                 Walker<V> wx(x, a.x.row, p.from + g.row(), col, kCh, g.down);
                 const int rows = static_cast<int>((count - g.row() + g.down - 1) / g.down);
-                const auto add = [&](const V &v) {
+                Run<T, kCh> run;
+                int left = rows;
+#pragma unroll 1
+                while (left >= kAhead) {
+                    const int many = left == rows ? kAhead : min(left, kRun) / kAhead * kAhead;
+#pragma unroll 1
+                    for (int it = 0; it < many; it += kAhead, wx.next(kAhead)) {
+                        V v[kAhead];
 #pragma unroll
-                    for (int i = 0; i < kCh; ++i) {
-                        const float d = v.at(i) - base.at(i);
-                        s1[i] += d;
-                        s2[i] += d * d;
+                        for (int k = 0; k < kAhead; ++k) { v[k] = wx.load(k); }
+                        if (left == rows) {
+#pragma unroll
+                            for (int i = 0; i < kCh; ++i) { run.base[i] = 0.25f * v[0].at(i) + 0.25f * v[1].at(i) + 0.25f * v[2].at(i) + 0.25f * v[3].at(i); }
+                        }
+#pragma unroll
+                        for (int k = 0; k < kAhead; ++k) { run.add(v[k]); }
                     }
-                };
-                int it = 0;
-                for (; it + kAhead <= rows; it += kAhead, wx.next(kAhead)) {
-                    V v[kAhead];
-#pragma unroll
-                    for (int k = 0; k < kAhead; ++k) { v[k] = wx.load(k); }
-#pragma unroll
-                    for (int k = 0; k < kAhead; ++k) {
-                        add(v[k]);
-                    }
+                    run.end(many, first, lines);
+                    left -= many;
                 }
-                for (; it < rows; ++it, wx.next(1)) {
-                    const V v = wx.load(0);
-                    add(v);
+                if (left > 0) {
+#pragma unroll 1
+                    for (int k = 0; k < left; ++k, wx.next(1)) {
+                        const V v = wx.load(0);
+                        if (k == 0 && left == rows) {
+#pragma unroll
+                            for (int i = 0; i < kCh; ++i) { run.base[i] = v.at(i); }
+                        }
+                        run.add(v);
+                    }
+                    run.end(left, first, lines);
                 }
             }
-            column_sums<kCh>(g, pass, p.width, s1, s2, lines, shares, total);
+            column_sums<kCh>(g, pass, p.width, lines, shares, total);
         }
-        __syncthreads();
         // ---- mean and sum of squared deviations of each group in the slice
         const double share = a.per_value * static_cast<double>(a.positions);
         if (cluster) { cluster_runs(); }
@@ -112,15 +158,15 @@ __global__ void __launch_bounds__(kNormThreads, 4) forward_kernel(NormArgs a)
     for (int pass = 0; pass < g.passes; ++pass) {
         const int col = g.column(pass);
         if (col >= g.columns || g.row() >= g.down) { continue; }
-        // (x - mean) * scale + bias as one multiply-add: either way what is lost is what 32 bits lose of mean * scale
+        // (x - mean) * scale + bias as one multiply-add, whose second term goes with the scale as it was rounded: what is lost is half
+        // a step of mean * scale.
         float scale[kCh], shift[kCh];
 #pragma unroll
         for (int i = 0; i < kCh; ++i) {
             const int c = col * kCh + i;
             const double2 st = total[c / a.per];
-            const double k = st.y * weight_of(a, p.c0 + c);
-            scale[i] = static_cast<float>(k);
-            shift[i] = static_cast<float>(bias_of(a, p.c0 + c) - st.x * k);
+            scale[i] = static_cast<float>(st.y * weight_of(a, p.c0 + c));
+            shift[i] = static_cast<float>(bias_of(a, p.c0 + c) - st.x * scale[i]);
         }
         Walker<V> wx(x, a.x.row, p.from + g.row(), col, kCh, g.down), wy(y, a.y.row, p.from + g.row(), col, kCh, g.down),
             wr = wy;

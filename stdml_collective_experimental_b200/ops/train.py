@@ -37,8 +37,8 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, res
     tensors (any row and image stride) are read where they lie, others are copied first; the
     result is channels last.  weight, bias: one value for each channel, of any of the three
     types; residual: as x.  activation: None, "relu", "silu", "gelu".  Statistics are taken
-    over the positions and channels of a group and kept in 64 bits; values next to the border
-    of "relu" are placed in 64."""
+    over the positions and channels of a group: in 32 bits over runs of 16 positions, about a mean
+    nearby, and in 64 beyond; values next to the border of "relu" are placed in 64."""
     return _native.fastcall().group_norm(x, residual, weight, bias, groups, eps,
                                          _code(_NORM_ACTS, activation, "activation"))
 

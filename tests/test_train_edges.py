@@ -1,0 +1,34 @@
+"""The operators of ops.train at inputs, sizes and uses where they can go wrong that test_train_ops.py does not reach: values far
+from the others, long sums, derivatives that they do not have, hooks, captures, waits that run out.  Bounds as there."""
+import pytest
+import torch
+from test_train_ops import BF16, F16, F32, channels_last, check_norm, cuda, gpu, rand
+
+from stdml_collective_experimental_b200 import ops
+
+
+# ------------------------------------------------------------------------- group norm: statistics
+@gpu
+@pytest.mark.parametrize("mean,spread", [(100.0, 1.0), (1000.3, 0.1), (1000.7, 0.0), (-3.0, 1.0)])
+@pytest.mark.parametrize("shape,groups", [((2, 8, 112, 112), 4), ((1, 32, 90, 77), 8), ((3, 512, 20, 20), 32), ((16, 8, 512, 512), 4)])
+@pytest.mark.parametrize("place", ["corner", "border", "scattered"])
+def test_group_norm_with_values_far_from_the_others(place, shape, groups, mean, spread):
+    """A masked or padded position, in the first place of an image or of a slice above all, takes no bits from the rest."""
+    x = channels_last(shape, 1, F32, spread, mean)
+    if place == "corner":
+        x[:, :, 0, 0] = 0
+    elif place == "border":
+        x[:, :, :, 0] = 0
+    else:
+        x.movedim(1, -1).view(shape[0], -1, shape[1])[:, ::257] = 0
+    check_norm(x, groups, rand(shape[1], 2, shift=1.0, scale=0.3), rand(shape[1], 3), 1e-5, "silu", None, channels_last(shape, 4, F32))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_group_norm_sums_over_many_positions(dtype):
+    """Of one and the same value, whose roundings would all point the same way: 1024 positions to a thread."""
+    shape = (10, 4, 1024, 1024)
+    x = channels_last(shape, 1, dtype)
+    dy = torch.full((shape[0], *shape[2:], shape[1]), 0.7, device=cuda, dtype=dtype).movedim(-1, 1)
+    check_norm(x, 2, rand(4, 2, shift=1.0), rand(4, 3), 1e-5, None, None, dy)
