@@ -8,6 +8,7 @@
 #include "train.hpp"
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -111,6 +112,15 @@ bool wanted(std::initializer_list<const Tensor *> all)
         if (t->defined() && t->requires_grad()) { return true; }
     }
     return false;
+}
+
+// A tangent would be dropped without a word where no gradient is wanted, and in the constants always.
+void no_tangent(const char *call, std::initializer_list<const Tensor *> all)
+{
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) { return; }
+    for (const Tensor *t : all) {
+        if (t->defined() && t->_fw_grad(0).defined()) { refuse(call, "has no forward-mode derivative: a tensor without a tangent expected"); }
+    }
 }
 
 // ------------------------------------------------------------ group normalisation
@@ -647,6 +657,7 @@ PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t n)
         const double eps = g.real();
         const long long act = g.integer();
         const WithoutGil free;
+        no_tangent(Norm::kCall, {&x, &residual, &weight, &bias});
         if (wanted({&x, &residual, &weight, &bias})) { return NormFunction::apply(x, maybe(residual), maybe(weight), maybe(bias), groups, eps, act); }
         Norm op;
         op.take(x, residual, weight, bias, groups, eps, static_cast<int>(act));
@@ -664,6 +675,7 @@ PyObject *distill_loss(PyObject *, PyObject *const *args, Py_ssize_t n)
         const double temperature = g.real(), alpha = g.real();
         const long long ignore = g.integer(), reduction = g.integer();
         const WithoutGil free;
+        no_tangent(Distill::kCall, {&logits, &top});
         if (top.requires_grad()) { refuse(Distill::kCall, "teacher_logits are constants: a tensor without gradient expected"); }
         if (wanted({&logits})) {
             return DistillFunction::apply(logits, top, index, maybe(labels), temperature, alpha, ignore, reduction);
@@ -684,6 +696,7 @@ PyObject *gated_linear(PyObject *, PyObject *const *args, Py_ssize_t n)
         const Tensor x = g.tensor(), wg = g.tensor(), wu = g.tensor(), bg = g.optional(), bu = g.optional();
         const long long act = g.integer();
         const WithoutGil free;
+        no_tangent(Gated::kCall, {&x, &wg, &wu, &bg, &bu});
         if (wanted({&x, &wg, &wu, &bg, &bu})) { return GatedFunction::apply(x, wg, wu, maybe(bg), maybe(bu), act); }
         Gated op;
         op.take(x, wg, wu, bg, bu, static_cast<int>(act));

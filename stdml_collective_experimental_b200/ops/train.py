@@ -3,7 +3,7 @@ activation and the shortcut of a residual block, ``gated_linear``, the gated pro
 of a feed-forward block, and ``distill_loss`` against a teacher's top logits.
 
 They run on the current stream of their tensors' GPU, whichever GPU is current, are
-differentiable once, and can be captured into a CUDA graph (after a first call outside of
+differentiable once (backward; tangents are refused), and can be captured into a CUDA graph (after a first call outside of
 one; forward and backward together, as autograd allows: no graph of the same leaves may live
 that was made on another stream).
 Workspaces and whatever is kept for the backward pass come from PyTorch's allocator; the

@@ -32,3 +32,27 @@ def test_group_norm_sums_over_many_positions(dtype):
     x = channels_last(shape, 1, dtype)
     dy = torch.full((shape[0], *shape[2:], shape[1]), 0.7, device=cuda, dtype=dtype).movedim(-1, 1)
     check_norm(x, 2, rand(4, 2, shift=1.0), rand(4, 3), 1e-5, None, None, dy)
+
+
+# ------------------------------------------------------------------------- derivatives that they do not have
+def calls():
+    """Of each operator: (what it takes, the call), on whatever device the tensors get."""
+    return [
+        ([torch.ones(2, 4, 3), torch.ones(4), torch.ones(4), torch.ones(2, 4, 3)],
+         lambda x, w, b, r: ops.group_norm(x, 2, w, b, residual=r)),
+        ([torch.ones(3, 8), torch.ones(5, 8), torch.ones(5, 8), torch.ones(5), torch.ones(5)], ops.gated_linear),
+        ([torch.ones(3, 8), torch.ones(3, 2)], lambda z, top: ops.distill_loss(z, top, torch.zeros(3, 2, dtype=torch.long, device=z.device))),
+    ]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_tangents_are_refused(native_lib, which):
+    from torch.autograd import forward_ad
+    args, call = calls()[which]
+    for i in range(len(args)):
+        with forward_ad.dual_level(), torch.no_grad():
+            dual = [forward_ad.make_dual(t, t) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(*dual)
+    with pytest.raises(ValueError, match="CUDA tensor expected"):
+        call(*args)
