@@ -11,6 +11,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -626,6 +627,8 @@ PyObject *guarded(F f)
     try {
         return THPVariable_Wrap(f());
     } catch (const Raised &) {
+    } catch (python_error &e) {  // of a hook on saved tensors: a checkpoint ends its second pass like that
+        e.restore();
     } catch (const c10::ValueError &e) {
         PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
     } catch (const c10::TypeError &e) {

@@ -56,3 +56,43 @@ def test_tangents_are_refused(native_lib, which):
                 call(*dual)
     with pytest.raises(ValueError, match="CUDA tensor expected"):
         call(*args)
+
+
+# ------------------------------------------------------------------------- hooks on saved tensors
+def on_gpu(which, dtype=F32):
+    """The same calls on a GPU: (leaves, the call)."""
+    if which == 0:
+        return ([channels_last((2, 8, 5, 5), 1, dtype), rand(8, 2), rand(8, 3), channels_last((2, 8, 5, 5), 4, dtype)],
+                lambda x, w, b, r: ops.group_norm(x, 2, w, b, activation="silu", residual=r))
+    if which == 1:
+        return [rand((9, 24), 1, dtype), rand((16, 24), 2, dtype), rand((16, 24), 3, dtype), rand(16, 4, dtype), rand(16, 5, dtype)], ops.gated_linear
+    top, index = torch.topk(rand((9, 40), 2), 5)
+    return [rand((9, 40), 1, dtype)], lambda z: ops.distill_loss(z, top, index, torch.arange(9, device=cuda), 2.0)
+
+
+@gpu
+@pytest.mark.parametrize("which", range(3))
+def test_an_exception_of_a_hook_is_the_callers(which):
+    class Mine(Exception):
+        pass
+
+    def pack(_):
+        raise Mine("packed")
+
+    args, call = on_gpu(which)
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t), pytest.raises(Mine, match="packed"):
+        call(*[t.requires_grad_() for t in args])
+    with torch.no_grad():
+        call(*args)
+
+
+@gpu
+@pytest.mark.parametrize("which", range(3))
+def test_checkpointed(which):
+    """The second pass of a checkpoint stops with an exception out of the last operator that saves anything."""
+    from torch.utils.checkpoint import checkpoint
+    args, call = on_gpu(which)
+    leaves = [t.requires_grad_() for t in args]
+    want = torch.autograd.grad(call(*leaves).square().sum(), leaves)
+    got = torch.autograd.grad(checkpoint(call, *leaves, use_reentrant=False).square().sum(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
