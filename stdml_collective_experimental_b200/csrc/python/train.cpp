@@ -404,10 +404,10 @@ struct Distill {
         const Tensor work = bytes_like(logits, stdmlc_distill_workspace(&d));
         d.workspace = work.data_ptr();
         done(stdmlc_distill_forward(&d, on.index(), on.stream()));
-        captured = stdmlc_stream_capturing(on.stream()) != 0;
+        capture = stdmlc_stream_capturing(on.stream());
         return {loss, stats};
     }
-    bool captured = false;
+    int64_t capture = 0;  // that the call is part of
 };
 
 struct DistillFunction : torch::autograd::Function<DistillFunction> {
@@ -426,7 +426,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
         ctx->saved_data["reduction"] = reduction;
         if (grad.defined()) {
             ctx->saved_data["grad"] = grad;
-            ctx->saved_data["captured"] = op.captured;
+            ctx->saved_data["capture"] = op.capture;
         }
         return loss;
     }
@@ -443,9 +443,8 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
         Tensor dlogits;
         const auto held = ctx->saved_data.find("grad");
         // The forward pass's gradient, for the first who asks.  It is multiplied in place, so a graph that is captured
-        // takes only one that its own replays write anew.
-        if (held != ctx->saved_data.end() &&
-            (stdmlc_stream_capturing(on.stream()) == 0) == !ctx->saved_data["captured"].toBool()) {
+        // takes only one that its own replays write anew: of the same capture.
+        if (held != ctx->saved_data.end() && stdmlc_stream_capturing(on.stream()) == ctx->saved_data["capture"].toInt()) {
             dlogits = held->second.toTensor();
             ctx->saved_data.erase("grad");
             done(stdmlc_distill_scale(dlogits.data_ptr(), dlogits.numel(), op.d.dt, dloss.data_ptr<float>(), on.index(), on.stream()));

@@ -75,7 +75,7 @@ long long stdmlc_distill_workspace(const stdmlc_distill *a);
 int stdmlc_distill_forward(const stdmlc_distill *a, int device, void *stream);
 int stdmlc_distill_backward(const stdmlc_distill *a, int device, void *stream);
 int stdmlc_distill_scale(void *grad, long long count, int dt, const float *by, int device, void *stream);
-int stdmlc_stream_capturing(void *stream); /* 1: a graph is being captured on it */
+long long stdmlc_stream_capturing(void *stream); /* the number of the capture that it is in; 0: none */
 
 /* h = act(g) * u, g = x w_gate^T + b_gate, u = x w_up^T + b_up. */
 typedef struct {

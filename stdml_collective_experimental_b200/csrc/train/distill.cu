@@ -614,9 +614,10 @@ extern "C" int stdmlc_distill_scale(void *grad, long long count, int dt, const f
     });
 }
 
-extern "C" int stdmlc_stream_capturing(void *stream)
+extern "C" long long stdmlc_stream_capturing(void *stream)
 {
     cudaStreamCaptureStatus how = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &how) != cudaSuccess) { (void)cudaGetLastError(); }
-    return how != cudaStreamCaptureStatusNone ? 1 : 0;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &how, &id) != cudaSuccess) { (void)cudaGetLastError(); }
+    return how != cudaStreamCaptureStatusNone ? static_cast<long long>(id) : 0;
 }

@@ -96,3 +96,32 @@ def test_checkpointed(which):
     want = torch.autograd.grad(call(*leaves).square().sum(), leaves)
     got = torch.autograd.grad(checkpoint(call, *leaves, use_reentrant=False).square().sum(), leaves)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------- distillation: the gradient of the forward pass
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_distill_loss_backward_captured_apart_and_replayed_again(dtype):
+    z = rand((17, 3001), 1, dtype).requires_grad_()
+    top, index = torch.topk(z.detach().float(), 10)
+    labels, up = torch.arange(17, device=cuda), torch.tensor(4.0, device=cuda)
+
+    def loss_of():
+        return ops.distill_loss(z, top, index, labels, 2.0)
+
+    first, = torch.autograd.grad(loss_of(), z, up)
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(forward):
+        loss = loss_of()
+    with torch.cuda.graph(backward, pool=forward.pool()):
+        dz, = torch.autograd.grad(loss, z, up)
+    for seed in (1, 5):
+        with torch.no_grad():
+            z.copy_(rand((17, 3001), seed, dtype))
+        want, = torch.autograd.grad(loss_of(), z, up)
+        forward.replay()
+        for _ in range(3):  # (an accumulation step that asks again)
+            backward.replay()
+            assert torch.equal(dz, want)
+    del first
