@@ -395,8 +395,7 @@ struct Distill {
         Tensor loss = d.reduction == 0 ? at::empty(rows, f32) : at::empty({}, f32);
         d.row_stats = stats.data_ptr<float>();
         d.loss = loss.data_ptr<float>();
-        // 16-bit numbers of a small exponent wait for what multiplies them: a loss scale saves them from nothing
-        // once they are rounded
+        // (f16 logits come with a loss scale, whose gradient is not one: theirs waits for the backward pass)
         if (with_grad && d.reduction != 0 && d.dt != 9) {
             grad = empty_grad();
             d.dlogits = grad.data_ptr();
@@ -442,21 +441,21 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
         const Tensor dloss = grads[0].to(at::kFloat).contiguous();
         Tensor dlogits;
         const auto held = ctx->saved_data.find("grad");
-        // The forward pass's gradient, for the first who asks.  It is multiplied in place, so a graph that is captured
-        // takes only one that its own replays write anew: of the same capture.
+        // The forward pass's gradient, for the first who asks: as it is for a loss of gradient one, which the kernel looks at.  For
+        // another it is written over, so a graph that is captured takes only one that its own replays write anew: of the same capture.
         if (held != ctx->saved_data.end() && stdmlc_stream_capturing(on.stream()) == ctx->saved_data["capture"].toInt()) {
             dlogits = held->second.toTensor();
             ctx->saved_data.erase("grad");
-            done(stdmlc_distill_scale(dlogits.data_ptr(), dlogits.numel(), op.d.dt, dloss.data_ptr<float>(), on.index(), on.stream()));
+            op.d.written = 1;
         } else {
             dlogits = op.empty_grad();
-            op.lay_out();
-            op.d.dloss = dloss.data_ptr<float>();
-            op.d.dloss_row = op.d.reduction == 0 ? 1 : 0;
-            op.d.row_stats = saved[4].data_ptr<float>();
-            op.d.dlogits = dlogits.data_ptr();
-            done(stdmlc_distill_backward(&op.d, on.index(), on.stream()));
         }
+        op.lay_out();
+        op.d.dloss = dloss.data_ptr<float>();
+        op.d.dloss_row = op.d.reduction == 0 ? 1 : 0;
+        op.d.row_stats = saved[4].data_ptr<float>();
+        op.d.dlogits = dlogits.data_ptr();
+        done(stdmlc_distill_backward(&op.d, on.index(), on.stream()));
         return {dlogits, {}, {}, {}, {}, {}, {}, {}};
     }
 };

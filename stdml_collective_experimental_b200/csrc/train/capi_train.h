@@ -67,14 +67,15 @@ typedef struct {
     const float *dloss; /* one value, or one of each row (dloss_row apart) */
     long long dloss_row;
     /* rows x classes, packed.  In a forward call (bf16 and f32, reductions to one value): null, or where to write the
-     * gradient of the loss, which stdmlc_distill_scale() multiplies by the loss's own gradient later. */
+     * gradient of the loss.  In a backward call where to write it; with `written` it has the forward call's already, which
+     * is what a loss of gradient one wants, and is written again for another. */
     void *dlogits;
+    int written;
 } stdmlc_distill;
 
 long long stdmlc_distill_workspace(const stdmlc_distill *a);
 int stdmlc_distill_forward(const stdmlc_distill *a, int device, void *stream);
 int stdmlc_distill_backward(const stdmlc_distill *a, int device, void *stream);
-int stdmlc_distill_scale(void *grad, long long count, int dt, const float *by, int device, void *stream);
 long long stdmlc_stream_capturing(void *stream); /* the number of the capture that it is in; 0: none */
 
 /* h = act(g) * u, g = x w_gate^T + b_gate, u = x w_up^T + b_up. */

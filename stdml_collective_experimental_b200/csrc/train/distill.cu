@@ -10,6 +10,8 @@
 // walks it once with running maximum and sums, and, where the caller wants gradients, a second time to write
 // them: the row comes from the L2 then, since the rows in work at a time are fewer than fit there.  The classes that
 // the teacher or the label names are corrected afterwards.
+#include <algorithm>
+
 #include "dispatch.cuh"
 #include "host.hpp"
 #include "ptx.cuh"
@@ -423,6 +425,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(Args a)
     if (threadIdx.x == 0) { *d.loss = static_cast<float>(sum); }
 }
 
+// The gradient of a loss of gradient d.dloss.  Where the forward pass has written that of a loss of gradient one (d.written), there is
+// nothing to do for one, and for another the whole of it is computed again: multiplied, it would be rounded twice.
 template <typename T, bool kHard, bool kSoft, int kPower>
 __global__ void __launch_bounds__(1024) grad_kernel(Args a)
 {
@@ -430,44 +434,27 @@ __global__ void __launch_bounds__(1024) grad_kernel(Args a)
     __shared__ float slots[33];
     const stdmlc_distill &d = a.d;
     const int parts = a.cluster, part = parts > 1 ? static_cast<int>(cta_rank()) : 0;
-    const long long r = blockIdx.x / parts;
-    const float *st = d.row_stats + kStats * r;
-    const float weight = st[4];
-    if (weight == 0.f) {
-        zero_row(static_cast<T *>(a.grad) + r * d.classes, d.classes, part, parts);
-        return;
-    }
-    const float up = weight * d.dloss[d.reduction == 0 ? r * d.dloss_row : 0];
-    float *prob = held;
-    int *cls = reinterpret_cast<int *>(held + d.top_count);
-    const float lp = part == 0 ? teacher_row(d, r, prob, cls, slots) : st[3];
-    if (part == 0) {
-        for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
-            prob[j] = cls[j] >= 0 && lp != -INFINITY ? expf(prob[j] - lp) : 0.f;
+    if (d.written != 0 && *d.dloss == 1.f) { return; }
+    for (long long r = blockIdx.x / parts; r < d.rows; r += gridDim.x / parts) {
+        const float *st = d.row_stats + kStats * r;
+        const float weight = st[4];
+        if (weight == 0.f) {
+            zero_row(static_cast<T *>(a.grad) + r * d.classes, d.classes, part, parts);
+            continue;
         }
-        __syncthreads();
+        const float up = weight * d.dloss[d.reduction == 0 ? r * d.dloss_row : 0];
+        float *prob = held;
+        int *cls = reinterpret_cast<int *>(held + d.top_count);
+        const float lp = part == 0 ? teacher_row(d, r, prob, cls, slots) : st[3];
+        if (part == 0) {
+            for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
+                prob[j] = cls[j] >= 0 && lp != -INFINITY ? expf(prob[j] - lp) : 0.f;
+            }
+            __syncthreads();
+        }
+        write_row<T, kHard, kSoft, kPower>(d, r, a.grad, up, st[0], st[1], st[2], lp, prob, cls, part, parts);
+        __syncthreads();  // (prob and cls are the next row's)
     }
-    write_row<T, kHard, kSoft, kPower>(d, r, a.grad, up, st[0], st[1], st[2], lp, prob, cls, part, parts);
-}
-
-// A gradient that the forward pass has written, times what came from above: nothing to do for one.
-template <typename T>
-__global__ void __launch_bounds__(512) scale_kernel(T *grad, long long many, const float *dloss)
-{
-    const float up = *dloss;
-    if (up == 1.f) { return; }
-    const long long first = blockIdx.x * 512ll + threadIdx.x, step = gridDim.x * 512ll;
-    constexpr int kPer = 16 / sizeof(T);
-    uint4 *v = reinterpret_cast<uint4 *>(grad);
-    for (long long i = first; i < many / kPer; i += step) {
-        const uint4 raw = v[i];
-        float f[kPer];
-        unpack16<T>(raw, f);
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) { f[k] *= up; }
-        v[i] = pack16<T>(f);
-    }
-    for (long long i = many / kPer * kPer + first; i < many; i += step) { grad[i] = from_f32<T>(to_f32(grad[i]) * up); }
 }
 
 void check(const stdmlc_distill *d)
@@ -522,10 +509,10 @@ void by_need(const stdmlc_distill &d, F f)
 }
 
 template <typename Kernel>
-void launch_rows(Kernel kernel, const Args &a, int threads, cudaStream_t s)
+void launch_rows(Kernel kernel, const Args &a, long long rows, int threads, cudaStream_t s)
 {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned int>(a.d.rows * a.cluster));
+    cfg.gridDim = dim3(static_cast<unsigned int>(rows * a.cluster));
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = 8 * static_cast<size_t>(a.d.top_count);
     cfg.stream = s;
@@ -574,7 +561,7 @@ extern "C" int stdmlc_distill_forward(const stdmlc_distill *d, int device, void 
         }
         by_dtype(d->dt, [&](auto t) {
             by_need(*d, [&](auto hard, auto soft, auto power) {
-                launch_rows(rows_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0, decltype(power)::value>, a, threads, s);
+                launch_rows(rows_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0, decltype(power)::value>, a, d->rows, threads, s);
             });
         });
     });
@@ -588,28 +575,20 @@ extern "C" int stdmlc_distill_backward(const stdmlc_distill *d, int device, void
         require(d->dloss != nullptr && d->dlogits != nullptr, "distill_loss: null operand");
         Args a{*d, nullptr, nullptr, 0, d->dlogits, 1};
         int threads;
+        require(d->written == 0 || d->reduction != 0, "distill_loss: no gradient in the forward pass here");
         launch_shape(*d, a.cluster, threads);
+        // Blocks that find nothing to do cost a launch of thousands some microseconds, so each takes several rows where there may be
+        // nothing: as many blocks as fit on the GPU twice (4096 rows of 256 KB: 5.5 us with four times as many).
+        long long rows = d->rows;
+        if (d->written != 0 && a.cluster == 1) {
+            const long long most = 2ll * sm_count() * (1024 / threads), each = (rows + most - 1) / most;
+            rows = (rows + each - 1) / each;
+        }
         by_dtype(d->dt, [&](auto t) {
             by_need(*d, [&](auto hard, auto soft, auto power) {
-                launch_rows(grad_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0, decltype(power)::value>, a, threads,
+                launch_rows(grad_kernel<decltype(t), decltype(hard)::value != 0, decltype(soft)::value != 0, decltype(power)::value>, a, rows, threads,
                             static_cast<cudaStream_t>(stream));
             });
-        });
-    });
-}
-
-extern "C" int stdmlc_distill_scale(void *grad, long long count, int dt, const float *by, int device, void *stream)
-{
-    return entry(device, [&] {
-        require(float_type(dt) && count >= 0, "distill_loss: bf16, f16 or f32 expected");
-        if (count == 0) { return; }
-        require(by != nullptr && grad != nullptr && reinterpret_cast<uintptr_t>(grad) % 16 == 0,
-                "distill_loss: a gradient on a 16-byte boundary expected");
-        by_dtype(dt, [&](auto t) {
-            using T = decltype(t);
-            const long long blocks = (count * static_cast<long long>(sizeof(T)) + 512 * 16 - 1) / (512 * 16), most = 4 * sm_count();
-            scale_kernel<T><<<static_cast<unsigned int>(blocks < most ? blocks : most), 512, 0, static_cast<cudaStream_t>(stream)>>>(
-                static_cast<T *>(grad), count, by);
         });
     });
 }

@@ -58,8 +58,8 @@ def distill_loss(logits, teacher_logits, teacher_index, labels=None, temperature
     gradient goes to the logits alone, in their type.
 
     With reduction "mean" or "sum", bf16 and f32 logits that want a gradient get it in the
-    forward pass already, for a loss of gradient 1; the backward pass multiplies it, where that
-    is another.  Under torch.no_grad() the loss alone is computed."""
+    forward pass already, for a loss of gradient 1; for another the backward pass computes it
+    again.  Under torch.no_grad() the loss alone is computed."""
     return _native.fastcall().distill_loss(logits, teacher_logits, teacher_index, labels,
                                            temperature, alpha, ignore_index,
                                            _code(_REDUCTIONS, reduction, "reduction"))

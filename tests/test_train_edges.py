@@ -2,7 +2,7 @@
 from the others, long sums, derivatives that they do not have, hooks, captures, waits that run out.  Bounds as there."""
 import pytest
 import torch
-from test_train_ops import BF16, F16, F32, channels_last, check_norm, cuda, gpu, rand
+from test_train_ops import BF16, F16, F32, U, channels_last, check_norm, cuda, gpu, plain_distill, rand, within
 
 from stdml_collective_experimental_b200 import ops
 
@@ -125,3 +125,24 @@ def test_distill_loss_backward_captured_apart_and_replayed_again(dtype):
             backward.replay()
             assert torch.equal(dz, want)
     del first
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("up", [0.75, 1 / 3, 24.0, 1.0, -1.0, 0.0])
+@pytest.mark.parametrize("rows,classes", [(17, 3001), (1500, 700), (3, 40000)])
+def test_distill_loss_gradient_is_rounded_once(rows, classes, up, dtype):
+    """Whatever the loss's own gradient is, the first backward pass over a graph gives the bits of the second, and those of the
+    definition but for what 32 bits lose and half a step of the logits' type."""
+    z = rand((rows, classes), 1, dtype, 2.0).requires_grad_()
+    top, index = torch.topk(z.detach().float() + rand((rows, classes), 2), 9)
+    labels = torch.arange(rows, device=cuda) % classes
+    labels[::5] = -100
+    loss = ops.distill_loss(z, top, index, labels, temperature=2.0, alpha=0.3)
+    first, = torch.autograd.grad(loss, z, torch.tensor(up, device=cuda), retain_graph=True)
+    second, = torch.autograd.grad(loss, z, torch.tensor(up, device=cuda))
+    assert torch.equal(first, second)
+    _, counts, grad, _, gsize = plain_distill(z.detach(), top, index, labels, 2.0, 0.3, -100)
+    each = abs(float(torch.tensor(up))) / float(counts.sum())
+    e = (classes / 128 + 64 + 8 * float(z.detach().abs().max())) * U  # (as check_distill)
+    within(first, grad * (each if up >= 0 else -each), gsize * each * (e + 16 * U))
