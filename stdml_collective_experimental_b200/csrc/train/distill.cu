@@ -385,7 +385,8 @@ __global__ void __launch_bounds__(1024) rows_kernel(Args a)
         float kl = 0;
         for (int j = threadIdx.x; j < d.top_count; j += blockDim.x) {
             const float logp = prob[j] - lp, p = cls[j] >= 0 ? expf(logp) : 0.f;
-            if (kSoft && lp != -INFINITY && cls[j] >= 0 && logp != -INFINITY) {
+            // (an entry whose weight has vanished has no term, wherever the student is: 0 log 0; NaN stays)
+            if (kSoft && lp != -INFINITY && cls[j] >= 0 && p != 0.f) {
                 kl += p * (logp - ((to_f32(z[cls[j]]) - most) * inv_t - log_soft));
             }
             prob[j] = lp != -INFINITY ? p : 0.f;

@@ -2,7 +2,7 @@
 from the others, long sums, derivatives that they do not have, hooks, captures, waits that run out.  Bounds as there."""
 import pytest
 import torch
-from test_train_ops import BF16, F16, F32, U, channels_last, check_norm, cuda, gpu, plain_distill, rand, within
+from test_train_ops import BF16, F16, F32, U, channels_last, check_distill, check_norm, cuda, gpu, plain_distill, rand, within
 
 from stdml_collective_experimental_b200 import ops
 
@@ -146,3 +146,18 @@ def test_distill_loss_gradient_is_rounded_once(rows, classes, up, dtype):
     each = abs(float(torch.tensor(up))) / float(counts.sum())
     e = (classes / 128 + 64 + 8 * float(z.detach().abs().max())) * U  # (as check_distill)
     within(first, grad * (each if up >= 0 else -each), gsize * each * (e + 16 * U))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("t", [1.0, 0.5])
+@pytest.mark.parametrize("low", [-300.0, -60000.0])
+def test_distill_loss_of_an_entry_without_weight_that_the_student_masks(low, t, dtype):
+    """A teacher's entry far below its first weighs exp(-300) or less: nothing, and a student that forbids the class is not
+    wrong."""
+    z, top, index = rand((4, 200), 1, dtype), rand((4, 3), 2, dtype), torch.tensor([[5, 9, 30]], device=cuda).repeat(4, 1)
+    top[1:, 1] = low
+    z[1, 9] = -torch.inf
+    z[2, 9] = torch.finfo(dtype).min
+    check_distill(z, top, index, None, t)
+    check_distill(z, top, index, torch.tensor([5, 30, 0, 199], device=cuda), t, 0.4)
