@@ -61,7 +61,7 @@ typedef struct {
     float temperature, alpha;
     int reduction;     /* 0: each row, 1: sum, 2: mean over the rows that count */
     float *loss;       /* one value, or one of each row */
-    float *row_stats;  /* [rows][5]: maximum, the two sums, the teacher's log-sum, weight of the row */
+    float *row_stats;  /* [rows][5]: maximum, the two sums, the teacher's maximum, weight of the row */
     void *workspace;   /* stdmlc_distill_workspace() bytes */
     /* backward */
     const float *dloss; /* one value, or one of each row (dloss_row apart) */

@@ -161,3 +161,24 @@ def test_distill_loss_of_an_entry_without_weight_that_the_student_masks(low, t, 
     z[2, 9] = torch.finfo(dtype).min
     check_distill(z, top, index, None, t)
     check_distill(z, top, index, torch.tensor([5, 30, 0, 199], device=cuda), t, 0.4)
+
+
+@gpu
+@pytest.mark.parametrize("t", [0.7, 1.0, 2.0, 3.0, 4.0])
+@pytest.mark.parametrize("rows,classes", [(256, 1000), (300, 30522), (2, 50001)])
+def test_distill_loss_in_f32_is_as_near_as_elementary_operations(rows, classes, t):
+    """Neither takes more than a subtraction, a quotient, an exponential, a sum and a product of 32 bits, so that neither is further
+    from 64 bits than the other but for chance, which over thousands of values is small."""
+    z = rand((rows, classes), 1, F32, 2.0).requires_grad_()
+    top, index = torch.topk(z.detach() + rand((rows, classes), 2), 5)
+    labels = torch.arange(rows, device=cuda)
+    dz, = torch.autograd.grad(ops.distill_loss(z, top, index, labels, t, 0.5, reduction="sum"), z)
+    exact = plain_distill(z.detach(), top, index, labels, t, 0.5, -100)[2]
+    with torch.no_grad():
+        p = torch.exp(top / t - (top / t).amax(1, keepdim=True))
+        plain = 0
+        for scale, at, off, weight in ((1.0, labels[:, None], 1.0, 0.5), (t, index, p / p.sum(1, keepdim=True), 0.5 * t)):
+            e = torch.exp(z / scale - (z / scale).amax(1, keepdim=True))
+            plain = plain + weight * (e / e.sum(1, keepdim=True)).scatter_add_(1, at, torch.zeros_like(at, dtype=F32) - off)
+    mine, theirs = (float((g.double() - exact).norm() / exact.norm()) for g in (dz, plain))
+    assert mine <= 1.5 * theirs, (mine, theirs)
