@@ -101,7 +101,7 @@ long long stdmlc_gated_workspace(const stdmlc_gated *a, int backward);
 int stdmlc_gated_forward(const stdmlc_gated *a, int device, void *stream);
 int stdmlc_gated_backward(const stdmlc_gated *a, int device, void *stream);
 
-/* Waits for the GPU's work.  *out: 0, or 1 where a bounded wait of an operator has run out since the last
+/* Waits for all of the GPU's work, on whatever stream (so not while one is captured).  *out: 0, or 1 where a bounded wait of an operator has run out since the last
  * question (its results are not complete). */
 int stdmlc_train_status(int device, int *out);
 

@@ -8,6 +8,7 @@
 // its epilogue.  32-bit operands are cut into three bf16 pieces of 8 bits each, which together are
 // the operand, and the six products of pieces that reach 2^-24 are summed.
 #include <algorithm>
+#include <mutex>
 
 #include "dispatch.cuh"
 #include "host.hpp"
@@ -17,7 +18,10 @@ namespace stdml::collective::train
 {
 namespace
 {
-__device__ unsigned int g_status;
+__device__ unsigned int g_status, g_taken;
+
+// Asked and cleared in one step, so that nothing is lost that is reported meanwhile.
+__global__ void take_status_kernel() { g_taken = atomicExch(&g_status, 0u); }
 
 // ------------------------------------------------------------ what the backward pass needs of g and u
 // Blocks of some columns of a row, both values together.  16-bit types: 24 bits of each, the upper 16 and the next 8
@@ -1016,12 +1020,12 @@ extern "C" int stdmlc_train_status(int device, int *out)
 {
     return entry(device, [&] {
         require(out != nullptr, "status: null output");
+        static std::mutex one_at_a_time;  // g_taken has one place
+        const std::lock_guard<std::mutex> lock(one_at_a_time);
+        cuda_ok(cudaDeviceSynchronize(), "status");  // (a copy alone waits for no stream that was made non-blocking)
+        take_status_kernel<<<1, 1>>>();
         unsigned int v = 0;
-        cuda_ok(cudaMemcpyFromSymbol(&v, g_status, sizeof v), "status");
-        if (v != 0) {
-            const unsigned int none = 0;
-            cuda_ok(cudaMemcpyToSymbol(g_status, &none, sizeof none), "status");
-        }
-        *out = static_cast<int>(v);
+        cuda_ok(cudaMemcpyFromSymbol(&v, g_taken, sizeof v), "status");
+        *out = v != 0 ? 1 : 0;
     });
 }

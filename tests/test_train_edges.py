@@ -182,3 +182,20 @@ def test_distill_loss_in_f32_is_as_near_as_elementary_operations(rows, classes, 
             plain = plain + weight * (e / e.sum(1, keepdim=True)).scatter_add_(1, at, torch.zeros_like(at, dtype=F32) - off)
     mine, theirs = (float((g.double() - exact).norm() / exact.norm()) for g in (dz, plain))
     assert mine <= 1.5 * theirs, (mine, theirs)
+
+
+# ------------------------------------------------------------------------- the report of waits that ran out
+@gpu
+def test_check_waits_for_every_stream():
+    args, call = on_gpu(1)
+    with torch.no_grad():
+        call(*args)  # (a kernel's first launch may wait by itself)
+    ops.check()
+    side, done = torch.cuda.Stream(), torch.cuda.Event()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.no_grad():
+        torch.cuda._sleep(1 << 30)  # (half a second of a kernel that waits for nobody)
+        call(*args)
+        done.record()
+    ops.check()
+    assert done.query()
