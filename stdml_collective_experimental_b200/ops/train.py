@@ -78,9 +78,13 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="gelu"):
 
 
 def check(device=None):
-    """Waits for a GPU's work and raises DeviceTimeoutError if a bounded wait inside one of these
-    operators has run out since the last question: its results are not complete then."""
-    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    """Waits for all work of a GPU (the current one, if none is named) and raises DeviceTimeoutError if
+    a bounded wait inside one of these operators has run out since the last question: its results are
+    not complete then.  Not while a graph is being captured."""
+    where = torch.device("cuda" if device is None else device)
+    if where.type != "cuda":
+        raise ValueError(f"check: CUDA device expected, got {where}")
+    index = torch.cuda.current_device() if where.index is None else where.index
     status = ctypes.c_int()
     _native.check(_native.lib().stdmlc_train_status(index, ctypes.byref(status)))
     if status.value:

@@ -199,3 +199,22 @@ def test_check_waits_for_every_stream():
         done.record()
     ops.check()
     assert done.query()
+
+
+def test_check_asks_the_gpu_that_is_meant(monkeypatch):
+    from stdml_collective_experimental_b200.ops import train
+    asked = []
+
+    class Lib:
+        @staticmethod
+        def stdmlc_train_status(index, _):
+            asked.append(index)
+            return 0
+
+    monkeypatch.setattr(train._native, "lib", lambda: Lib)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    for device in (None, "cuda", torch.device("cuda"), "cuda:0", torch.device("cuda", 1), 2):
+        ops.check(device)
+    assert asked == [3, 3, 3, 0, 1, 2]
+    with pytest.raises(ValueError, match="CUDA device"):
+        ops.check("cpu")
