@@ -26,7 +26,7 @@ import torch.distributed as dist
 
 from .. import DeviceSession
 from ..models.resnet import ResNet50
-from ..ops import distill_loss
+from ..ops import check, distill_loss
 from ..parallel.ddp import DataParallel
 
 
@@ -112,6 +112,7 @@ def run_mode(mode, args, sess, rank, world, dev):
         ms = float(t.item())
     if ddp is not None:
         sess.check()
+    check(dev)  # the models' operators
     out = {"mode": mode, "model": args.model, "n_gpus": world, "batch_per_gpu": args.batch,
            "ms_per_step": ms, "images_per_s": world * args.batch / (ms * 1e-3), "loss": float(loss)}
     out.update({k: v for k, v in (("norm", args.norm), ("ffn", args.ffn), ("teacher", args.teacher))

@@ -218,3 +218,16 @@ def test_check_asks_the_gpu_that_is_meant(monkeypatch):
     assert asked == [3, 3, 3, 0, 1, 2]
     with pytest.raises(ValueError, match="CUDA device"):
         ops.check("cpu")
+
+
+@gpu
+@pytest.mark.parametrize("model", ["resnet50", "bert-base"])
+def test_the_benchmark_asks_after_its_steps(monkeypatch, model):
+    import argparse
+
+    from stdml_collective_experimental_b200.benchmarks import resnet50_dp
+    asked = []
+    monkeypatch.setattr(resnet50_dp, "check", asked.append, raising=False)
+    args = argparse.Namespace(model=model, batch=2, seq=8, steps=1, warmup=1, buckets=2, norm="group", ffn="gated", teacher=4)
+    out = resnet50_dp.run_mode("local", args, None, 0, 1, cuda)
+    assert asked == [cuda] and out["loss"] == out["loss"]
