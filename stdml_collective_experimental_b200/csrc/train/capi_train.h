@@ -94,6 +94,9 @@ typedef struct {
     const void *dh;
     long long dh_row;
     void *dx, *dw_gate, *dw_up, *db_gate, *db_up; /* packed */
+    /* How long a wait inside a kernel may last before it gives up, which stdmlc_train_status() reports.  0: ten
+     * seconds; negative: none may, and nothing is computed (a call of more than four tokens, or backward, gives up at once). */
+    long long wait_limit_ns;
 } stdmlc_gated;
 
 long long stdmlc_gated_saved(const stdmlc_gated *a);

@@ -626,6 +626,11 @@ unsigned int *status_word()
     return static_cast<unsigned int *>(p);
 }
 
+unsigned long long wait_limit(const stdmlc_gated *a)
+{
+    return a->wait_limit_ns == 0 ? 10ull * 1000 * 1000 * 1000 : a->wait_limit_ns < 0 ? 0 : static_cast<unsigned long long>(a->wait_limit_ns);
+}
+
 // Sizes of a product, without its operands.
 Product sizes(long long m, long long n, long long reduction, int halves, int z, bool two_b)
 {
@@ -905,6 +910,7 @@ void forward(const stdmlc_gated *a, cudaStream_t s)
     p.b[1] = f.w_up.as.map(map_type(a->dt), f.width / kCtas);
     set_kind(p, a->dt, f.width);
     f.w.status = status_word();
+    f.w.wait_ns = wait_limit(a);
     f.scratch.clear(f.w, s);
     by_dtype(a->dt, [&](auto t) {
         using T = decltype(t);
@@ -964,6 +970,7 @@ void backward(const stdmlc_gated *a, cudaStream_t s)
             for (const void *p : {a->dw_gate, a->dw_up}) { tile.vec = tile.vec && (p == nullptr || aligned_rows(p, a->hidden, a->dt)); }
         }
         b.w.status = status_word();
+        b.w.wait_ns = wait_limit(a);
         b.scratch.clear(b.w, s);
         launch<sizeof(T) == 4>(b.w, tile, b.clusters, b.width, s);
     });

@@ -59,11 +59,12 @@ struct Work {
     int own_part;
     unsigned int *tickets;  // zero: [tile][CTA of the pair][epilogue warp]
     unsigned int *status;
+    unsigned long long wait_ns;  // how long a wait may last; 0: the kernel gives up with its first loads under way
 };
 
 // Why a kernel gave up: a wait ran out.
 constexpr unsigned int kWaitRanOut = 1;
-constexpr unsigned long long kWaitLimitNs = 10ull * 1000 * 1000 * 1000;
+constexpr unsigned long long kSettleNs = 1000 * 1000 * 1000;
 
 __device__ __forceinline__ unsigned long long clock_ns()
 {
@@ -72,22 +73,60 @@ __device__ __forceinline__ unsigned long long clock_ns()
     return t;
 }
 
-// False: the block gives up (`dead` in its shared memory says so to all its warps).
-static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *dead, unsigned int *status)
+__device__ __forceinline__ void give_up(volatile int *dead, unsigned int *status)
 {
-    const unsigned long long t0 = clock_ns();
-    for (unsigned int spins = 0; spins < (1u << 28); ++spins) {
-        if (bar_try(bar, parity)) { return true; }
-        if (*dead != 0) { return false; }
-        if ((spins & 63u) == 63u && clock_ns() - t0 > kWaitLimitNs) { break; }
-    }
     *dead = 1;
     atomicExch(status, kWaitRanOut);
+}
+
+// False: the block gives up (`dead` in its shared memory says so to all its warps).
+static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *dead, const Work &w)
+{
+    const unsigned long long limit = w.wait_ns, t0 = clock_ns();
+    for (unsigned int spins = 0; limit != 0 && spins < (1u << 28); ++spins) {
+        if (bar_try(bar, parity)) { return true; }
+        if (*dead != 0) { return false; }
+        if ((spins & 63u) == 63u && clock_ns() - t0 > limit) { break; }
+    }
+    give_up(dead, w.status);
     return false;
 }
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *dead, unsigned int *status)
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *dead, const Work &w)
 {
-    return bar_try(bar, parity) || wait_slow(bar, parity, dead, status);
+    return bar_try(bar, parity) || wait_slow(bar, parity, dead, w);
+}
+
+// What a CTA has asked for when its roles have ended.
+struct Asked {
+    int dead;
+    int loads;         // steps whose copies it has asked for
+    int steps, sums;   // (of the pair's first CTA) steps, and tiles or chunks of them, whose products it has asked for
+};
+
+// Where either CTA of a pair has given up: what is under way into their shared and tensor memory ends before they do.  One thread of
+// each; both CTAs know what either has asked for.  The waits are bounded too, and nothing comes of one that runs out.
+static __device__ __noinline__ void settle(uint32_t full, uint32_t empty, uint32_t summed, int stages, uint32_t stage_bytes, bool first,
+                                           const volatile Asked &mine, const volatile Asked &other)
+{
+    const auto wait = [](uint32_t bar, int phase) {
+        const unsigned long long t0 = clock_ns();
+        while (!bar_try(bar, phase & 1) && clock_ns() - t0 < kSettleNs) {}
+    };
+    // products arrive at the barriers of both
+    const int steps = first ? mine.steps : other.steps, sums = first ? mine.sums : other.sums;
+    for (int i = max(0, steps - stages); i < steps; ++i) { wait(empty + 8 * (i % stages), i / stages); }
+    for (int i = max(0, sums - 2); i < sums; ++i) { wait(summed + 8 * (i & 1), i / 2); }
+    if (!first) { return; }
+    // The copies of both arrive at the first one's.  A CTA that is ahead of the other in a stage has the other's bytes to go without
+    // (its own arrival counts on them), or, as the second, no arrival that counts on its own.
+    for (int s = 0; s < stages; ++s) {
+        const auto last = [&](int loads) { return loads > s ? (loads - 1 - s) / stages : -1; };  // use of this stage
+        const int a = last(mine.loads), b = last(other.loads);
+        if (a < 0 && b < 0) { continue; }
+        if (a > b) { bar_forgo(full + 8 * s, stage_bytes); }
+        if (b > a) { bar_expect(full + 8 * s, stage_bytes); }
+        wait(full + 8 * s, max(a, b));
+    }
 }
 
 // What a unit is: a part of a tile of a product.
@@ -213,7 +252,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
 {
     extern __shared__ unsigned char raw[];
     __shared__ uint32_t tmem_at;
-    __shared__ int dead_flag;
+    __shared__ Asked asked[2];  // this CTA's, the other's
     using S = Shape<kN, kWide>;
     constexpr int kStages = S::kStages, kStageBytes = S::kStageBytes;
     constexpr uint32_t kColumns = 2 * kN;  // of tensor memory: one tile is summed while the other is taken
@@ -222,12 +261,12 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
     uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kEpilogueWarps * kStagingBytes);
     const uint32_t ring_at = smem_at(ring), full = smem_at(bars), empty = full + 8 * kStages,
                    summed = empty + 8 * kStages, taken = summed + 16;
-    volatile int *dead = &dead_flag;
+    volatile int *dead = &asked[0].dead;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cta_rank();
 
     if (threadIdx.x == 0) {
-        dead_flag = 0;
+        asked[0] = Asked{};
         for (int i = 0; i < kStages; ++i) {
             bar_init(full + 8 * i, 1);
             bar_init(empty + 8 * i, 1);
@@ -257,7 +296,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
             const int n0 = u.n * (p.two_b ? kN / 2 : kN) + (p.two_b ? 0 : kN / 2 * static_cast<int>(rank));
             for (int step = u.from; step < u.to; ++step, ++it) {
                 const int st = it % kStages;
-                ok = it < kStages || wait_for(empty + 8 * st, (it / kStages - 1) & 1, dead, w.status);
+                ok = it < kStages || wait_for(empty + 8 * st, (it / kStages - 1) & 1, dead, w);
                 if (!ok) { break; }
                 const uint32_t bar = full + 8 * st, at_a = ring_at + st * kStageBytes, at_b = at_a + S::kOf * kChunkA;
                 if (rank == 0) { bar_expect(bar, kCtas * kStageBytes); }
@@ -284,12 +323,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
         }
         // The copies asked for end before the block does: with the products that read them (an arrival on `empty`).
         for (int i = max(0, it - kStages); i < it; ++i) {
-            if (!wait_for(empty + 8 * (i % kStages), (i / kStages) & 1, dead, w.status)) { break; }
+            if (!wait_for(empty + 8 * (i % kStages), (i / kStages) & 1, dead, w)) { break; }
         }
+        asked[0].loads = it;
     } else if (warp == 1 && lane == 0 && rank == 0) {
         // ---- products
-        int it = 0, round = 0;
-        bool ok = true;
+        int it = 0, round = 0, sums = 0;
+        bool ok = w.wait_ns != 0;
+        if (!ok) { give_up(dead, w.status); }
         for (int i = mine; ok && i < w.units; i += workers) {
             const Unit u = unit_at(w, i);
             const Product &p = w.product[u.product];
@@ -300,14 +341,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
             const int chunk = kWide ? w.chunk : u.to - u.from;
             for (int c = u.from; ok && c < u.to; c += chunk, ++round) {
                 const int buf = round & 1;
-                ok = round < 2 || wait_for(taken + 8 * buf, (round / 2 - 1) & 1, dead, w.status);
+                ok = round < 2 || wait_for(taken + 8 * buf, (round / 2 - 1) & 1, dead, w);
                 if (!ok) { break; }
                 tmem_after_sync();
                 const uint32_t d = tmem + buf * kN;
                 const int steps = min(c + chunk, u.to) - c;
                 for (int k = 0; k < steps; ++k, ++it) {
                     const int st = it % kStages;
-                    ok = wait_for(full + 8 * st, (it / kStages) & 1, dead, w.status);
+                    ok = wait_for(full + 8 * st, (it / kStages) & 1, dead, w);
                     if (!ok) { break; }
                     tmem_after_sync();
                     const uint32_t at_a = ring_at + st * kStageBytes, at_b = at_a + S::kOf * kChunkA;
@@ -322,9 +363,14 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
                     }
                     mma_commit(empty + 8 * st);
                 }
-                if (ok) { mma_commit(summed + 8 * buf); }
+                if (ok) {
+                    mma_commit(summed + 8 * buf);
+                    ++sums;
+                }
             }
         }
+        asked[0].steps = it;
+        asked[0].sums = sums;
     } else if (warp >= 4) {
         // ---- epilogue
         const int quarter = warp & 3, slice = (warp - 4) >> 2;
@@ -346,7 +392,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
                 for (int j = 0; j < S::kValues; ++j) { sum[j] = 0.f; }
                 for (int c = u.from; c < u.to; c += w.chunk, ++round) {
                     const int buf = round & 1;
-                    ok = __all_sync(0xffffffffu, wait_for(summed + 8 * buf, (round / 2) & 1, dead, w.status));
+                    ok = __all_sync(0xffffffffu, wait_for(summed + 8 * buf, (round / 2) & 1, dead, w));
                     if (!ok) { break; }
                     tmem_after_sync();
 #pragma unroll
@@ -366,7 +412,7 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
                 for (int j = 0; j < S::kValues; ++j) { __stcg(part + 32 * j, sum[j]); }
             } else {
                 const int buf = round++ & 1;
-                ok = __all_sync(0xffffffffu, wait_for(summed + 8 * buf, ((round - 1) / 2) & 1, dead, w.status));
+                ok = __all_sync(0xffffffffu, wait_for(summed + 8 * buf, ((round - 1) / 2) & 1, dead, w));
                 if (!ok) { break; }
                 tmem_after_sync();
                 const FromTensorMemory<kN> from{lanes + buf * kN, two_b, slice, taken + 8 * buf};
@@ -405,8 +451,17 @@ __global__ void __cluster_dims__(kCtas, 1, 1) __launch_bounds__(kProductThreads,
     __syncwarp();
     tmem_before_sync();
     __syncthreads();
+    if (threadIdx.x < 4) {
+        send_word(reinterpret_cast<volatile int *>(&asked[1]) + threadIdx.x, rank ^ 1u, reinterpret_cast<volatile int *>(&asked[0])[threadIdx.x]);
+    }
     cluster_sync();
     tmem_after_sync();
+    if (*dead != 0 || *static_cast<volatile int *>(&asked[1].dead) != 0) {  // (the same in both CTAs)
+        if (threadIdx.x == 0) { settle(full, empty, summed, kStages, kStageBytes, rank == 0, asked[0], asked[1]); }
+        __syncthreads();
+        cluster_sync();
+        tmem_after_sync();
+    }
     if (warp == 2) { tmem_free(tmem, kColumns); }
 }
 }  // namespace stdml::collective::train

@@ -38,6 +38,18 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// Bytes that will not come count as if they had.
+__device__ __forceinline__ void bar_forgo(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// To the same place in a CTA of the cluster.
+__device__ __forceinline__ void send_word(const volatile int *place, uint32_t cta, int v)
+{
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_at(const_cast<const int *>(place))), "r"(cta));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
 // On the barrier at the same place in the cluster's first CTA.  Orders nothing: a release would wait for the stores under
 // way (a third of the time of an epilogue).
 __device__ __forceinline__ void bar_arrive_first(uint32_t bar)

@@ -1,8 +1,10 @@
 """The operators of ops.train at inputs, sizes and uses where they can go wrong that test_train_ops.py does not reach: values far
 from the others, long sums, derivatives that they do not have, hooks, captures, waits that run out.  Bounds as there."""
+import ctypes
+
 import pytest
 import torch
-from test_train_ops import BF16, F16, F32, U, channels_last, check_distill, check_norm, cuda, gpu, plain_distill, rand, within
+from test_train_ops import BF16, F16, F32, U, channels_last, check_distill, check_norm, cuda, gated_inputs, gpu, plain_distill, rand, within
 
 from stdml_collective_experimental_b200 import ops
 
@@ -231,3 +233,54 @@ def test_the_benchmark_asks_after_its_steps(monkeypatch, model):
     args = argparse.Namespace(model=model, batch=2, seq=8, steps=1, warmup=1, buckets=2, norm="group", ffn="gated", teacher=4)
     out = resnet50_dp.run_mode("local", args, None, 0, 1, cuda)
     assert asked == [cuda] and out["loss"] == out["loss"]
+
+
+class GatedCall(ctypes.Structure):
+    """stdmlc_gated of capi_train.h."""
+    _fields_ = [("x", ctypes.c_void_p), ("x_row", ctypes.c_longlong), ("w_gate", ctypes.c_void_p), ("w_up", ctypes.c_void_p),
+                ("w_gate_row", ctypes.c_longlong), ("w_up_row", ctypes.c_longlong), ("b_gate", ctypes.c_void_p),
+                ("b_up", ctypes.c_void_p), ("h", ctypes.c_void_p), ("tokens", ctypes.c_longlong), ("hidden", ctypes.c_longlong),
+                ("ffn", ctypes.c_longlong), ("dt", ctypes.c_int), ("act", ctypes.c_int), ("saved", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("dh", ctypes.c_void_p), ("dh_row", ctypes.c_longlong), ("dx", ctypes.c_void_p),
+                ("dw_gate", ctypes.c_void_p), ("dw_up", ctypes.c_void_p), ("db_gate", ctypes.c_void_p), ("db_up", ctypes.c_void_p),
+                ("wait_limit_ns", ctypes.c_longlong)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tokens,hidden,ffn", [(77, 64, 96), (300, 520, 264), (1024, 384, 512), (2100, 768, 2048)])
+def test_gated_linear_reports_a_wait_that_may_not_last(native_lib, tokens, hidden, ffn, dtype):
+    """Through the C ABI, whose callers may limit the waits: the kernel gives up with its first loads under way, says so, and the
+    next call is whole."""
+    from stdml_collective_experimental_b200 import _native
+    lib = _native.lib()
+    lib.stdmlc_gated_saved.restype = lib.stdmlc_gated_workspace.restype = ctypes.c_longlong
+    x, wg, wu, _, _, dh = gated_inputs(tokens, hidden, ffn, dtype, False)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    h = ops.gated_linear(*leaves)
+    want = [h, *torch.autograd.grad(h, leaves, dh)]
+    outs = [torch.zeros_like(t) for t in want]
+    a = GatedCall(x=x.data_ptr(), x_row=hidden, w_gate=wg.data_ptr(), w_up=wu.data_ptr(), w_gate_row=hidden, w_up_row=hidden,
+                  h=outs[0].data_ptr(), tokens=tokens, hidden=hidden, ffn=ffn, dt=8 if dtype == BF16 else 10, act=3, dh=dh.data_ptr(),
+                  dh_row=ffn, dx=outs[1].data_ptr(), dw_gate=outs[2].data_ptr(), dw_up=outs[3].data_ptr())
+    saved = torch.empty(lib.stdmlc_gated_saved(ctypes.byref(a)), dtype=torch.uint8, device=cuda)
+    a.saved = saved.data_ptr()
+
+    def run(backward, limit):
+        work = torch.empty(lib.stdmlc_gated_workspace(ctypes.byref(a), backward), dtype=torch.uint8, device=cuda)
+        a.workspace, a.wait_limit_ns = work.data_ptr(), limit
+        f = lib.stdmlc_gated_backward if backward else lib.stdmlc_gated_forward
+        _native.check(f(ctypes.byref(a), 0, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        torch.cuda.synchronize()
+
+    ops.check()
+    for backward in (0, 1):
+        run(backward, -1)
+        assert not any(o.any() for o in (outs[1:] if backward else outs))
+        with pytest.raises(_native.DeviceTimeoutError, match="ran out"):
+            ops.check()
+        ops.check()  # (once)
+        run(backward, 1_000_000_000)
+        run(backward, 0)
+        ops.check()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want[:4 if backward else 1]))
