@@ -80,20 +80,20 @@ __device__ __forceinline__ void give_up(volatile int *dead, unsigned int *status
 }
 
 // False: the block gives up (`dead` in its shared memory says so to all its warps).
-static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *dead, const Work &w)
+static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *dead, unsigned int *status, unsigned long long limit)
 {
-    const unsigned long long limit = w.wait_ns, t0 = clock_ns();
+    const unsigned long long t0 = clock_ns();
     for (unsigned int spins = 0; limit != 0 && spins < (1u << 28); ++spins) {
         if (bar_try(bar, parity)) { return true; }
         if (*dead != 0) { return false; }
         if ((spins & 63u) == 63u && clock_ns() - t0 > limit) { break; }
     }
-    give_up(dead, w.status);
+    give_up(dead, status);
     return false;
 }
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *dead, const Work &w)
 {
-    return bar_try(bar, parity) || wait_slow(bar, parity, dead, w);
+    return bar_try(bar, parity) || wait_slow(bar, parity, dead, w.status, w.wait_ns);
 }
 
 // What a CTA has asked for when its roles have ended.
