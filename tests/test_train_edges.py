@@ -284,3 +284,21 @@ def test_gated_linear_reports_a_wait_that_may_not_last(native_lib, tokens, hidde
         run(backward, 0)
         ops.check()
         assert all(torch.equal(o, w) for o, w in zip(outs, want[:4 if backward else 1]))
+
+
+# ------------------------------------------------------------------------- gelu left of zero
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens", [4, 257])
+def test_gelu_of_16_bits_is_near_where_it_is_small(tokens, dtype):
+    """Relative to its own size, which vanishes like exp(-z^2 / 2): 2^-14 of it and half a step.  (5.2e-6 of the fit, three roundings
+    of z^2 / 2 in an exponent of up to 104 powers of two, two quotients: 1.9e-5.)"""
+    z = -torch.linspace(0, 12, 16 * tokens, device=cuda).to(dtype).view(tokens, 16)
+    one, nothing = torch.ones(16, device=cuda, dtype=dtype), torch.zeros(16, 16, device=cuda, dtype=dtype)
+    x = z.clone().requires_grad_()
+    h = ops.gated_linear(x, torch.eye(16, device=cuda, dtype=dtype), nothing, 0 * one, one, activation="gelu")  # gelu(z) * 1
+    z = z.double()
+    phi, cdf = torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5, 0.5 * torch.special.erfc(-z / 2 ** 0.5)
+    within(h, z * cdf, 2.0 ** -14 * (z * cdf).abs())
+    dz, = torch.autograd.grad(h, x, torch.ones_like(h))
+    within(dz, cdf + z * phi, 2.0 ** -14 * (cdf + z.abs() * phi))
