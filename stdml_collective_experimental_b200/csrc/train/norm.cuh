@@ -222,9 +222,9 @@ __device__ __forceinline__ double2 published(const NormArgs &a, const Part &p, c
 void norm_forward_launch(const NormArgs &n, int dt, int vector, int act, cudaStream_t s);
 void norm_backward_launch(const NormArgs &n, int dt, int vector, int act, cudaStream_t s);
 
-// One launch of clusters, or one for each walk.
+// One launch of clusters, or one for each walk (the second only where there are `results` beyond sums).
 template <typename Kernel>
-void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, cudaStream_t s)
+void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, bool results, cudaStream_t s)
 {
     const long long blocks = n.images * n.chunks * n.slices;
     // lines of sums, first values, shares of the lines, totals of channels, sums of groups (of all slices)
@@ -233,7 +233,7 @@ void norm_walks(Kernel kernel, NormArgs n, int channels_per_thread, cudaStream_t
     // (the most that any sizes take, always: another thread may be about to launch the same kernel with more)
     cuda_ok(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10), "shared memory");
     for (int walk : {1, 2}) {
-        if (n.walks == 3 && walk == 2) { return; }
+        if (walk == 2 && (n.walks == 3 || !results)) { return; }
         NormArgs args = n;
         args.walks = n.walks == 3 ? 3 : walk;
         cudaLaunchConfig_t cfg{};

@@ -8,20 +8,20 @@ namespace
 constexpr int kAhead = 2;  // rows that a thread has on their way
 constexpr int kRun = 64;   // rows whose sums are taken in 32 bits, before 64 take over
 
-// Factors of a thread's channels (four at most: with eight they would not leave room for two blocks on an SM).
+// Factors of a thread's channels (four at most: with eight they would not leave room for four blocks on an SM).
 // z = x * scale + shift [+ r]; below `near` (and what r adds) its sign is in doubt.
 template <int kCh>
 struct Factors {
     float mean[kCh], scale[kCh], shift[kCh], near[kCh];
 };
 
-// dz of a thread's channels in a row, and x - mean.
 // z where 32 bits leave its sign in doubt.
 __device__ __noinline__ float placed(float x, float add, double mean, double rstd, float w, float b)
 {
     return static_cast<float>((x - mean) * rstd * w + b + add);
 }
 
+// dz of a thread's channels in a row, and x - mean.
 template <typename T, int kCh, int kAct, bool kResidual>
 __device__ __forceinline__ void grad_z(const NormArgs &a, const Part &p, int col, const Factors<kCh> &f, const double2 *stats,
                                        const Vec<T, kCh> &x, const Vec<T, kCh> &r, const Vec<T, kCh> &dy, float (&dz)[kCh], float (&off)[kCh])
@@ -280,10 +280,11 @@ __global__ void __launch_bounds__(1024) params_kernel(const float *sums, long lo
 template <typename T, int kCh, int kAct>
 void backward(const NormArgs &n, cudaStream_t s)
 {
+    const bool results = n.dx.ptr != nullptr || n.dr.ptr != nullptr;
     if constexpr (kAct != STDMLC_ACT_NONE) {
-        if (n.r.ptr != nullptr) { return norm_walks(backward_kernel<T, kCh, kAct, true>, n, kCh, s); }
+        if (n.r.ptr != nullptr) { return norm_walks(backward_kernel<T, kCh, kAct, true>, n, kCh, results, s); }
     }
-    norm_walks(backward_kernel<T, kCh, kAct, false>, n, kCh, s);
+    norm_walks(backward_kernel<T, kCh, kAct, false>, n, kCh, results, s);
 }
 }  // namespace
 

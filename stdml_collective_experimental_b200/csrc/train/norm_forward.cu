@@ -215,9 +215,9 @@ template <typename T, int kCh, int kAct>
 void forward(const NormArgs &n, cudaStream_t s)
 {
     if (n.r.ptr != nullptr) {
-        norm_walks(forward_kernel<T, kCh, kAct, true>, n, kCh, s);
+        norm_walks(forward_kernel<T, kCh, kAct, true>, n, kCh, true, s);
     } else {
-        norm_walks(forward_kernel<T, kCh, kAct, false>, n, kCh, s);
+        norm_walks(forward_kernel<T, kCh, kAct, false>, n, kCh, true, s);
     }
 }
 }  // namespace

@@ -302,3 +302,25 @@ def test_gelu_of_16_bits_is_near_where_it_is_small(tokens, dtype):
     within(h, z * cdf, 2.0 ** -14 * (z * cdf).abs())
     dz, = torch.autograd.grad(h, x, torch.ones_like(h))
     within(dz, cdf + z * phi, 2.0 ** -14 * (cdf + z.abs() * phi))
+
+
+# ------------------------------------------------------------------------- group norm: gradients that nobody wants
+@gpu
+def test_group_norm_walks_once_for_parameters_alone():
+    """One large image is worked on in two launches, of which the second writes dx: for weight and bias the first is all."""
+    from torch.profiler import ProfilerActivity, profile
+    x, dy = (channels_last((1, 8, 201, 307), s, F32) for s in (1, 2))
+    w, b = rand(8, 3, shift=1.0).requires_grad_(), rand(8, 4).requires_grad_()
+
+    def launches(leaves):
+        y = ops.group_norm(x, 4, w, b, activation="silu", residual=dy)
+        torch.cuda.synchronize()
+        with profile(activities=[ProfilerActivity.CUDA]) as p:
+            torch.autograd.grad(y, leaves, dy)
+            torch.cuda.synchronize()
+        return sum("backward_kernel" in e.name for e in p.events())
+
+    launches([w, b])
+    assert launches([w, b]) == 1 and launches([w]) == 1
+    x.requires_grad_()
+    assert launches([x, w, b]) == 2
