@@ -99,6 +99,9 @@ Tensor bytes_like(const Tensor &t, long long n)
     return at::empty({n}, t.options().dtype(at::kByte).requires_grad(false).memory_format(std::nullopt));
 }
 
+// Memory that holds the values' negatives (a view of a conjugate's imaginary part) is not read as it lies.
+Tensor plain(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 void *ptr_of(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // Operands that a call may lack: autograd's Function knows them as empty optionals, the code here as undefined tensors.
@@ -265,7 +268,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
                 static_cast<int>(ctx->saved_data["act"].toInt()));
         const OnDevice on(Norm::kCall, op.x, {&grads[0]});
         op.lay_out();
-        const Tensor dy = in_rows(grads[0], &op.a.dy);
+        const Tensor dy = in_rows(plain(grads[0]), &op.a.dy);
         op.a.stats = stats.data_ptr<double>();
         Tensor dx, dres, dw, db;
         size_t edge = 0;  // (autograd counts the operands that there are)
@@ -438,7 +441,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
                 ctx->saved_data["alpha"].toDouble(), ctx->saved_data["ignore"].toInt(),
                 static_cast<int>(ctx->saved_data["reduction"].toInt()));
         const OnDevice on(Distill::kCall, op.logits, {&grads[0]});
-        const Tensor dloss = grads[0].to(at::kFloat).contiguous();
+        const Tensor dloss = plain(grads[0]).to(at::kFloat).contiguous();
         Tensor dlogits;
         const auto held = ctx->saved_data.find("grad");
         // The forward pass's gradient, for the first who asks: as it is for a loss of gradient one, which the kernel looks at.  For
@@ -554,7 +557,7 @@ struct GatedFunction : torch::autograd::Function<GatedFunction> {
         op.take(saved[0], saved[1], saved[2], saved[3], saved[4], static_cast<int>(ctx->saved_data["act"].toInt()));
         const OnDevice on(Gated::kCall, op.x, {&grads[0]});
         op.lay_out();
-        const Tensor dh = matrix_of(grads[0], &op.a.dh, &op.a.dh_row);
+        const Tensor dh = matrix_of(plain(grads[0]), &op.a.dh, &op.a.dh_row);
         op.a.saved = saved[5].data_ptr();
         const auto packed = saved[0].options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
         tensor_list out(6);
@@ -592,7 +595,7 @@ struct Args {
         PyObject *o = a[i++];
         if (o == Py_None) { return {}; }
         if (!THPVariable_Check(o)) { refuse_type(call, std::string("tensor expected, got ") + Py_TYPE(o)->tp_name); }
-        return THPVariable_Unpack(o);
+        return plain(THPVariable_Unpack(o));
     }
     Tensor tensor()
     {

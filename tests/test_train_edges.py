@@ -324,3 +324,24 @@ def test_group_norm_walks_once_for_parameters_alone():
     assert launches([w, b]) == 1 and launches([w]) == 1
     x.requires_grad_()
     assert launches([x, w, b]) == 2
+
+
+# ------------------------------------------------------------------------- views of negatives
+@gpu
+@pytest.mark.parametrize("which", range(3))
+def test_memory_that_holds_negatives(which):
+    """Imaginary parts of conjugates are views with a sign of their own, as operands and as gradients."""
+    args, call = on_gpu(which)
+    leaves = [t.requires_grad_() for t in args]
+    y = call(*leaves)
+    dy = torch.randn_like(y)
+    want = [y, *torch.autograd.grad(y, leaves, dy)]
+    theirs = [torch._neg_view(-t.detach()) for t in args]
+    assert all(t.is_neg() for t in theirs)
+    with torch.no_grad():
+        assert torch.equal(call(*theirs), y)
+    for t in theirs:
+        t.requires_grad_()
+    y = call(*theirs)
+    got = [y, *torch.autograd.grad(y, theirs, torch._neg_view(-dy))]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
