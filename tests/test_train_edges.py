@@ -4,7 +4,8 @@ import ctypes
 
 import pytest
 import torch
-from test_train_ops import BF16, F16, F32, U, channels_last, check_distill, check_norm, cuda, gated_inputs, gpu, plain_distill, rand, within
+from test_train_ops import (BF16, F16, F32, U, channels_last, check_distill, check_gated, check_norm, cuda, gated_inputs, gpu,
+                            plain_distill, rand, within)
 
 from stdml_collective_experimental_b200 import ops
 
@@ -345,3 +346,19 @@ def test_memory_that_holds_negatives(which):
     y = call(*theirs)
     got = [y, *torch.autograd.grad(y, theirs, torch._neg_view(-dy))]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------- gated projection: the wide tiles
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens,hidden,ffn", [(4096, 768, 2048), (2100, 768, 2048), (1037, 1000, 2730), (2561, 520, 1300), (700, 2048, 5000)])
+def test_gated_linear_in_wide_tiles(tokens, hidden, ffn, dtype):
+    """Sizes of use: tiles 256 wide, more of them than there are pairs of SMs (tensor memory is taken in turns), more than eight
+    tile rows (bands), parts of long reductions."""
+    from torch.profiler import ProfilerActivity, profile
+    *ins, dh = gated_inputs(tokens, hidden, ffn, dtype, bias=tokens % 2 == 0)
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        check_gated(*ins, ["gelu", "silu", "gelu_tanh"][tokens % 3], dh)
+        torch.cuda.synchronize()
+    names = [e.name for e in p.events() if "product_kernel" in e.name]
+    assert len(names) == 2 and any("<false, 256," in n for n in names), names
