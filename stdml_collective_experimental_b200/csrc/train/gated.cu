@@ -34,6 +34,17 @@ struct Saved {
     __host__ __device__ static long long row_bytes(long long ffn) { return (ffn + kCols - 1) / kCols * kBytes; }
 };
 
+// ------------------------------------------------------------ the range of dg and du
+// dg and du are rounded to the operands' type for the tensor cores, half a step of it each: an error of the size of a result's own rounding, and not
+// more in sums of them, where it is of either sign.  (As two 16-bit pieces each they would take the gradients' products twice.)  In f16 they would
+// also overflow where dh u does, and vanish where a sum over many tokens does not: they are multiplied by a power of two that
+// puts the largest at 2^14, which the results are divided by in 32 bits.  So values down to 2^-28 of the largest keep all their bits.
+__device__ __forceinline__ int scale_exponent(unsigned int most)  // of what `most`, the bits of a float, is multiplied by
+{
+    return most == 0u ? 0 : min(126, 14 - (static_cast<int>(most >> 23) - 127));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<unsigned int>(e + 127) << 23); }
+
 // ------------------------------------------------------------ results of a tile
 // An epilogue warp has 32 rows of a tile, one to a thread; through 32 rows of 128 bytes in shared memory they reach
 // global memory 32 bytes and more in a row (stores of 16 bytes from 32 rows at a time took longer than the products).
@@ -198,6 +209,7 @@ struct GatedTile {
 template <typename T>
 struct PlainTile {
     T *out[2][2];  // [product][z]
+    const unsigned int *most;  // f16: what dg and du were scaled by
     bool vec;
 
     template <int kN, typename Source>
@@ -212,11 +224,16 @@ struct PlainTile {
             from.done();
             return;
         }
+        const float by = std::is_same_v<T, __half> ? power_of_two(-scale_exponent(__ldg(most))) : 1.f;
 #pragma unroll
         for (int b = 0; b < kCols / 16; ++b) {
             float v[16];
             from.load(b, v);
             from.loaded(v);
+            if constexpr (std::is_same_v<T, __half>) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { v[i] *= by; }
+            }
             put16<T>(mem, threadIdx.x & 31, b * static_cast<int>(sizeof(T)), v);
         }
         from.done();
@@ -311,6 +328,7 @@ struct GateGrad {
     long long tokens, ffn, pitch;
     uint16_t *d;      // [gate, up][pieces][tokens][pitch]
     float *partial;   // [row blocks][gate, up][ffn]; null: no sums
+    unsigned int *most;  // f16: bits of a bound of |dg| and |du|
     bool vec;
 };
 
@@ -362,9 +380,38 @@ struct GateGradRow {
     }
 };
 
+constexpr int kMostRows = 16;  // of a block (1037 x 2730: with 64 of them 8.4 us)
+
+// a.most, which is zero: |act'| <= 1.13 and |act(g)| <= |g|.  What is not finite stays so, and bounds nothing.
+template <typename T>
+__global__ void __launch_bounds__(256) gate_most_kernel(GateGrad a)
+{
+    const int across = static_cast<int>((a.ffn + kGradCols - 1) / kGradCols), down = blockIdx.x / across;
+    const long long col = (blockIdx.x - down * across) * static_cast<long long>(kGradCols) + 8 * (threadIdx.x & 31);
+    const long long first = down * static_cast<long long>(kMostRows), end = min(first + kMostRows, a.tokens);
+    float most = 0;
+    if (col < a.ffn) {
+#pragma unroll 2
+        for (long long r = first + (threadIdx.x >> 5); r < end; r += 8) {
+            GateGradRow<T> row;
+            row.load(a, r, col);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float g = row.value(row.g, make_uint2(0, 0), i), u = row.value(row.u, make_uint2(0, 0), i);
+                // (the upper bits alone: 1 % less at most)
+                const float v = fabsf(to_f32(row.dh[i])) * fmaxf(1.15f * fabsf(u), 1.02f * fabsf(g));
+                if (col + i < a.ffn && v > most && v < INFINITY) { most = v; }
+            }
+        }
+    }
+    most = warp_max(most);
+    if ((threadIdx.x & 31) == 0 && most > 0.f) { atomicMax(a.most, __float_as_uint(most)); }
+}
+
 template <typename T, int kAct>
 __global__ void __launch_bounds__(256) gate_grad_kernel(GateGrad a)
 {
+    const float scale = std::is_same_v<T, __half> ? power_of_two(scale_exponent(*a.most)) : 1.f;
     __shared__ float sums[2][8][kGradCols];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int across = static_cast<int>((a.ffn + kGradCols - 1) / kGradCols), down = blockIdx.x / across;
@@ -400,8 +447,8 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(GateGrad a)
 #pragma unroll
                     for (int j = 0; j < kPieces; ++j) { out[1][j][i] = piece[j]; }
                 } else {
-                    both[0][i] = dg;
-                    both[1][i] = du;
+                    both[0][i] = std::is_same_v<T, __half> ? dg * scale : dg;
+                    both[1][i] = std::is_same_v<T, __half> ? du * scale : du;
                 }
             }
             if constexpr (sizeof(T) == 2) {
@@ -724,11 +771,12 @@ int cut_tiles(Work &w, int clusters, bool wide)
 
 long long tiles_of(const Product &p) { return static_cast<long long>(p.m_tiles) * p.n_tiles * p.z; }
 
-// Memory of a launch's own: parts and tickets (null where nothing is split).
+// Memory of a launch's own: parts and tickets (none where nothing is split), and words that begin as zero like them.
 struct Scratch {
-    long long tickets = 0;
+    long long tickets = 0, words;
+    unsigned int *most;
 
-    Scratch(Work &w, int clusters, int width, bool wide, Bump &work)
+    Scratch(Work &w, int clusters, int width, bool wide, Bump &work, int more = 0)
     {
         bool split = false;
         for (int q = 0; q < w.products; ++q) {
@@ -736,12 +784,14 @@ struct Scratch {
             split = split || w.product[q].split > 1;
         }
         if (!split) { tickets = 0; }
-        w.tickets = work.take<unsigned int>(tickets);
+        words = tickets + more;
+        w.tickets = work.take<unsigned int>(words);
+        most = w.tickets + tickets;
         w.parts = work.take<float>((w.own_part + (wide ? clusters : 0)) * (width == 256 ? Shape<256, false>::kPart : Shape<128, true>::kPart));
     }
     void clear(const Work &w, cudaStream_t s) const
     {
-        if (tickets > 0) { cuda_ok(cudaMemsetAsync(w.tickets, 0, 4 * tickets, s), "cudaMemsetAsync"); }
+        if (words > 0) { cuda_ok(cudaMemsetAsync(w.tickets, 0, 4 * words, s), "cudaMemsetAsync"); }
     }
 };
 
@@ -836,7 +886,7 @@ struct Backward : Operands {
     Scratch scratch;
 
     explicit Backward(const stdmlc_gated *a) : Operands(a), d(grads(a)), partial(work.take<float>(2 * row_blocks(a) * a->ffn)),
-          scratch{plan(a), clusters, width, a->dt == kF32, work}
+          scratch{plan(a), clusters, width, a->dt == kF32, work, a->dt == kF16 ? 1 : 0}
     {
     }
 
@@ -929,13 +979,18 @@ void backward(const stdmlc_gated *a, cudaStream_t s)
     Backward b(a);
     const bool sums = a->db_gate != nullptr || a->db_up != nullptr;
     const GateGrad gg{a->dh, a->dh_row, static_cast<const unsigned char *>(a->saved), a->tokens, a->ffn, b.d.pitch,
-                      static_cast<uint16_t *>(const_cast<void *>(b.d.ptr)), sums ? b.partial : nullptr,
+                      static_cast<uint16_t *>(const_cast<void *>(b.d.ptr)), sums ? b.partial : nullptr, b.scratch.most,
                       aligned_rows(a->dh, a->dh_row, a->dt) && a->ffn * element_size(a->dt) % 16 == 0};
     const CUtensorMapDataType type = map_type(a->dt);
+    b.scratch.clear(b.w, s);
     by_dtype(a->dt, [&](auto t) {
         using T = decltype(t);
+        const long long across = (a->ffn + kGradCols - 1) / kGradCols, grid = across * row_blocks(a);
+        if constexpr (std::is_same_v<T, __half>) {
+            const long long down = (a->tokens + kMostRows - 1) / kMostRows;
+            gate_most_kernel<T><<<static_cast<unsigned int>(across * down), 256, 0, s>>>(gg);
+        }
         by_gate(a->act, [&](auto k) {
-            const long long grid = (a->ffn + kGradCols - 1) / kGradCols * row_blocks(a);
             gate_grad_kernel<T, decltype(k)::value><<<static_cast<unsigned int>(grid), 256, 0, s>>>(gg);
         });
         if (sums) {
@@ -950,7 +1005,7 @@ void backward(const stdmlc_gated *a, cudaStream_t s)
         } else {
             pack({&b.x}, s);
         }
-        PlainTile<T> tile{{{nullptr, nullptr}, {nullptr, nullptr}}, true};
+        PlainTile<T> tile{{{nullptr, nullptr}, {nullptr, nullptr}}, b.scratch.most, true};
         if (b.dx >= 0) {
             Product &p = b.w.product[b.dx];
             p.a = b.d.map(type, kTileM);
@@ -971,7 +1026,6 @@ void backward(const stdmlc_gated *a, cudaStream_t s)
         }
         b.w.status = status_word();
         b.w.wait_ns = wait_limit(a);
-        b.scratch.clear(b.w, s);
         launch<sizeof(T) == 4>(b.w, tile, b.clusters, b.width, s);
     });
 }

@@ -4,7 +4,7 @@ import ctypes
 
 import pytest
 import torch
-from test_train_ops import (BF16, F16, F32, U, channels_last, check_distill, check_gated, check_norm, cuda, gated_inputs, gpu,
+from test_train_ops import (ACTS, BF16, F16, F32, U, channels_last, check_distill, check_gated, check_norm, cuda, gated_inputs, gpu,
                             plain_distill, rand, within)
 
 from stdml_collective_experimental_b200 import ops
@@ -362,3 +362,48 @@ def test_gated_linear_in_wide_tiles(tokens, hidden, ffn, dtype):
         torch.cuda.synchronize()
     names = [e.name for e in p.events() if "product_kernel" in e.name]
     assert len(names) == 2 and any("<false, 256," in n for n in names), names
+
+
+# ------------------------------------------------------------------------- gated projection: the range of f16
+@gpu
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("tokens,hidden,ffn", [(3, 64, 72), (20, 64, 64), (600, 72, 264)])
+@pytest.mark.parametrize("x_size,w_size,up_size,dh_size", [
+    (1e-3, 1e-3, 30.0, 2e4),          # dh u is beyond 65504, its products with w and x are not
+    (100.0, 1e-3, 2.0 ** -9, 2.0 ** -16),  # dh u is below 2^-24, its sums with x over the tokens are not
+    (1.0, 0.1, 1.0, 1.0),
+])
+def test_gated_linear_in_f16_beyond_the_range_of_what_it_multiplies(x_size, w_size, up_size, dh_size, tokens, hidden, ffn, act):
+    x, wg, wu, bg, bu, dh = gated_inputs(tokens, hidden, ffn, F32, True)
+    x, dh = (x * x_size).to(F16), (dh.clamp(-3, 3) * dh_size).to(F16)
+    wg, wu = ((w.sign() * w_size * (0.5 + 0.1 * w.abs())).to(F16) for w in (wg, wu))
+    bg, bu = bg.to(F16), (up_size * (1 + 0.1 * bu)).to(F16)
+    dh[1] = 0  # (and a row of nothing)
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    grads = torch.autograd.grad(ops.gated_linear(*leaves, bg, bu, activation=act), leaves, dh)
+    X, G, W, D = (t.detach().double() for t in (x, wg, wu, dh))
+    g, u = (X @ G.t() + bg.double()).requires_grad_(), X @ W.t() + bu.double()
+    a = ACTS[act](g)
+    da, = torch.autograd.grad(a.sum(), g)
+    dg, du = D * u * da, D * a.detach()
+    # half a step of f16 for dg and du, 2^-15 for each of g and u as they are kept (the derivatives follow by 1.2 at most), some 2^-20 for
+    # sums of few hundred terms in 32 bits: below 2^-11 (1 + 1/4) of the terms' sizes
+    rel = 1.25 * 2.0 ** -11
+    eg = D.abs() * (u.abs() * (da.abs() + 2.0 ** -4) + 2.0 ** -4)  # (2^-15 of g and u, 2^-4 of the bound)
+    eu = D.abs() * (a.detach().abs() + 2.0 ** -4 * g.detach().abs())
+    within(grads[0], dg @ G + du @ W, rel * (eg @ G.abs() + eu @ W.abs()))
+    within(grads[1], dg.t() @ X, rel * (eg.t() @ X.abs()))
+    within(grads[2], du.t() @ X, rel * (eu.t() @ X.abs()))
+    assert all(t.isfinite().all() for t in grads)
+
+
+@gpu
+def test_gated_linear_in_f16_infinite_gradients_stay_in_their_rows():
+    x, wg, wu, bg, bu, dh = gated_inputs(140, 96, 80, F16, True)
+    x = x.requires_grad_()
+    want, = torch.autograd.grad(ops.gated_linear(x, wg, wu, bg, bu), x, dh)
+    dh[3, 7], dh[9, 1] = torch.inf, torch.nan
+    got, = torch.autograd.grad(ops.gated_linear(x, wg, wu, bg, bu), x, dh)
+    rest = torch.ones(140, dtype=torch.bool, device=cuda)
+    rest[[3, 9]] = False
+    assert torch.equal(got[rest], want[rest]) and not got[3].isfinite().any() and got[9].isnan().all()
