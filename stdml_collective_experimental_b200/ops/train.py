@@ -72,7 +72,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="gelu"):
     x: (..., hidden) of bf16, f16 or f32; weights (ffn, hidden) and biases (ffn,) of the same
     type, rows of any stride (the halves of one fused weight, for instance); both biases or
     none.  activation: "gelu", "gelu_tanh", "silu".  Products are summed in 32 bits; f32
-    operands keep their 24 bits (an infinity among them comes out as NaN)."""
+    operands keep their 24 bits (an infinity among them comes out as NaN).  For gradients of
+    16-bit types those of the two projections are rounded to the type once (in f16 after
+    scaling, so that none leaves its range), and multiplied in it."""
     return _native.fastcall().gated_linear(x, w_gate, w_up, b_gate, b_up,
                                            _code(_GATES, activation, "activation"))
 
