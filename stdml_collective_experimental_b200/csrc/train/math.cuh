@@ -115,10 +115,10 @@ __device__ __forceinline__ float fast_rcp(float v)
 constexpr float kLog2E = 1.4426950408889634f;
 
 // z's activation and the derivative there, for results of type T.  32-bit results take CUDA's functions.  For 16-bit
-// ones the exponential and the quotient are the hardware's, and erfc(x) = 2 exp(-x^2) poly(1 / (1 + 0.44 x)), whose exponential the
+// ones the exponential and the quotient are the hardware's, and erfc(x) = 2 exp(-x^2) poly(1 / (1 + 0.33 x)), whose exponential the
 // derivative needs anyway.  The polynomial was fitted to exp(x^2) erfc(x) / 2 for the least maximum of the relative error over x up to 9.5,
-// 5.2e-6; with what 32 bits lose, a value left of zero is 1.5e-5 off at most down to z = -12, 2^-5 of half a step of f16.  (The kernels
-// would otherwise spend longer on erf than on memory.)
+// 8.2e-8; with what 32 bits lose, gelu is 4 x 2^-24 |z| off at most, and left of zero 2e-6 of itself down to z = -6 and 8e-6 to -12 (half a
+// step of f16 is 2.4e-4 at least).  (The kernels would otherwise spend longer on erf than on memory.)
 template <typename T, int kAct>
 __device__ __forceinline__ void act_both(float z, float &a, float &d)
 {
@@ -140,8 +140,9 @@ __device__ __forceinline__ void act_both(float z, float &a, float &d)
     } else if constexpr (kAct == STDMLC_ACT_GELU) {
         // q = erfc(|z| / sqrt 2) / 2: z (1 - q) right of zero, z q left of it.  (Beyond 30, where q is 0, |z| does not
         // matter; an infinity would.)
-        const float x = fminf(fabsf(z), 30.f), t = fast_rcp(1.f + 0.44f * kSqrtHalf * x), e = fast_exp2(-0.5f * kLog2E * z * z);
-        const float q = e * t * (0.12428051f + t * (0.12128476f + t * (0.13179333f + t * (0.020365113f + t * (0.17532669f - t * 0.07305298f)))));
+        const float x = fminf(fabsf(z), 30.f), t = fast_rcp(1.f + 0.33f * kSqrtHalf * x), e = fast_exp2(-0.5f * kLog2E * z * z);
+        const float q = e * t * (0.0931830449f + t * (0.0914187618f + t * (0.100961095f + t * (0.022507869f + t * (0.206266189f +
+                                 t * (-0.177714604f + t * (0.231341345f - t * 0.0679637408f)))))));
         a = fmaxf(z, 0.f) - x * q;
         d = (z < 0.f ? q : 1.f - q) + z * (kGauss * e);
     } else {

@@ -407,3 +407,18 @@ def test_gated_linear_in_f16_infinite_gradients_stay_in_their_rows():
     rest = torch.ones(140, dtype=torch.bool, device=cuda)
     rest[[3, 9]] = False
     assert torch.equal(got[rest], want[rest]) and not got[3].isfinite().any() and got[9].isnan().all()
+
+
+@gpu
+def test_gelu_of_every_f16_number():
+    """4 U |z| of the formula in 32 bits, an exponential and a quotient of the hardware (4 U each of a value that is below |z| / 2); left of
+    zero in relation to the value: 1.5e-6, and z^2 / 2 times 1.5 roundings of the exponent."""
+    z = torch.arange(0x4800 + 1, dtype=torch.int16, device=cuda).view(F16)  # 0 .. 8
+    z = torch.cat([z, -z])
+    z = z[:z.numel() // 16 * 16].view(-1, 16)
+    one, nothing = torch.ones(16, device=cuda, dtype=F16), torch.zeros(16, 16, device=cuda, dtype=F16)
+    with torch.no_grad():
+        h = ops.gated_linear(z, torch.eye(16, device=cuda, dtype=F16), nothing, 0 * one, one, activation="gelu")
+    z = z.double()
+    cdf = 0.5 * torch.special.erfc(-z / 2 ** 0.5)
+    within(h, z * cdf, torch.where(z > 0, 8 * U * z, (1.5e-6 + 1.5 * U * z * z) * (z * cdf).abs()))
