@@ -104,6 +104,16 @@ Tensor plain(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg
 
 void *ptr_of(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// A tensor without memory of its own (a subclass that wraps others, a fake one) would pass for an operand that is not there.
+void has_memory(const char *call, std::initializer_list<const Tensor *> all)
+{
+    for (const Tensor *t : all) {
+        if (t->defined() && t->numel() > 0 && (!t->has_storage() || t->storage().data() == nullptr)) {
+            refuse_type(call, "a plain tensor expected, got one without memory of its own");
+        }
+    }
+}
+
 // Operands that a call may lack: autograd's Function knows them as empty optionals, the code here as undefined tensors.
 using Maybe = std::optional<Tensor>;
 Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
@@ -661,6 +671,7 @@ PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t n)
         const double eps = g.real();
         const long long act = g.integer();
         const WithoutGil free;
+        has_memory(Norm::kCall, {&x, &residual, &weight, &bias});
         no_tangent(Norm::kCall, {&x, &residual, &weight, &bias});
         if (wanted({&x, &residual, &weight, &bias})) { return NormFunction::apply(x, maybe(residual), maybe(weight), maybe(bias), groups, eps, act); }
         Norm op;
@@ -679,6 +690,7 @@ PyObject *distill_loss(PyObject *, PyObject *const *args, Py_ssize_t n)
         const double temperature = g.real(), alpha = g.real();
         const long long ignore = g.integer(), reduction = g.integer();
         const WithoutGil free;
+        has_memory(Distill::kCall, {&logits, &top, &index, &labels});
         no_tangent(Distill::kCall, {&logits, &top});
         if (top.requires_grad()) { refuse(Distill::kCall, "teacher_logits are constants: a tensor without gradient expected"); }
         if (wanted({&logits})) {
@@ -700,6 +712,7 @@ PyObject *gated_linear(PyObject *, PyObject *const *args, Py_ssize_t n)
         const Tensor x = g.tensor(), wg = g.tensor(), wu = g.tensor(), bg = g.optional(), bu = g.optional();
         const long long act = g.integer();
         const WithoutGil free;
+        has_memory(Gated::kCall, {&x, &wg, &wu, &bg, &bu});
         no_tangent(Gated::kCall, {&x, &wg, &wu, &bg, &bu});
         if (wanted({&x, &wg, &wu, &bg, &bu})) { return GatedFunction::apply(x, wg, wu, maybe(bg), maybe(bu), act); }
         Gated op;

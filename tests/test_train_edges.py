@@ -422,3 +422,34 @@ def test_gelu_of_every_f16_number():
     z = z.double()
     cdf = 0.5 * torch.special.erfc(-z / 2 ** 0.5)
     within(h, z * cdf, torch.where(z > 0, 8 * U * z, (1.5e-6 + 1.5 * U * z * z) * (z * cdf).abs()))
+
+
+# ------------------------------------------------------------------------- tensors that are not plain
+class Wrapped(torch.Tensor):
+    """A subclass around another tensor, without memory of its own."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device, strides=inner.stride())
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} was asked of a wrapper")
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_tensors_without_memory_are_refused(native_lib, which):
+    args, call = calls()[which]
+    with torch.no_grad():
+        for i in range(len(args)):
+            with pytest.raises(TypeError, match="without memory"):
+                call(*[Wrapped(t) if j == i else t for j, t in enumerate(args)])
+
+
+@gpu
+@pytest.mark.parametrize("which", range(3))
+def test_tensors_without_memory_are_refused_on_a_gpu(which):
+    args, call = on_gpu(which)
+    for i in range(len(args)):
+        with torch.no_grad(), pytest.raises(TypeError, match="without memory"):
+            call(*[Wrapped(t) if j == i else t for j, t in enumerate(args)])
